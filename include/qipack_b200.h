@@ -427,6 +427,137 @@ int qi_shard_put_slice(void *context, void *const *y_copies, int copies, int out
  * completes on any rank's stream (a four-byte NCCL all-reduce). */
 int qi_shard_barrier(void *context, void *stream);
 
+/* ---- between the packed linears: norms, a cache of keys and values, attention ------------------------------
+ *
+ * What a transformer block computes besides its linears, for serving (no gradients): the norms around a block with the
+ * block's gate, a paged cache of keys and values in 8 bits, attention over it, and the upkeep of its pages. The
+ * reference keeps its prefix cache in float16 and contiguous, and norms and gates are kernels of their own
+ * (qwen_image_cuda/src/transformer.cplus:748-818, qwen_image_cuda/cuda/ops.cu:37-118, flash.cu:52-244).
+ *
+ * Conventions as above. What only the device knows (lengths, offsets, page numbers) is checked there: a kernel that
+ * meets something unsound reads and writes nothing through it and records 0x0006Cxxx in the status word
+ * (qi_kernel_status). Nothing here allocates, waits or keeps state: every call may be captured in a graph. */
+
+/* The pool of pages. Codes uint8 [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned; scales float32
+ * [layers][pages][kv_heads][page_tokens / 16], one for 16 consecutive tokens of one head: value = (code - 128) * scale.
+ * page_tokens 16, 32, 64, 128 or 256; head_dim 64 or 128. Nothing has to be cleared before its first use. */
+typedef struct {
+    void *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    int layers, pages, page_tokens, kv_heads, head_dim;
+} qi_kv_cache;
+
+/* Which pages hold which tokens, the same for all layers: token t of sequence s is in page
+ * table[s * table_pages + t / page_tokens] (-1: none), lengths[s] tokens in all; references[p] sequences hold page p
+ * (0: it is free). An empty pool is lengths 0, references 0, table -1. table_pages <= 2^19. */
+typedef struct {
+    int *table, *lengths, *references;
+    int sequences, table_pages;
+} qi_kv_pages;
+
+/* A ragged batch: entry b is the LAST offsets[b + 1] - offsets[b] tokens of sequence slots[b] (slots NULL: of sequence b),
+ * whose rows begin at row offsets[b] of the token arrays. offsets[0] = 0; `tokens` rows in all and `most` for one entry are
+ * bounds that the host knows; entries <= 65535. No sequence may be named twice where a call writes. */
+typedef struct {
+    const int *slots, *offsets;
+    int entries, tokens, most;
+} qi_kv_batch;
+
+/* Writes new tokens into layer `layer`: row r of k and v [tokens, kv_heads, head_dim], ld_k and ld_v elements between rows
+ * (multiples of 16 bytes), dtype QI_DTYPE_F32 or QI_DTYPE_F16. Their pages were reserved (qi_kv_pages_reserve_ex), so
+ * lengths already count them, and no other sequence holds those pages. A block of 16 tokens and one head has
+ *   scale = max |x| / 127 of its new tokens, or the scale of its earlier tokens if that is more,
+ *   code  = rint(x / scale) + 128, earlier tokens again as rint((code - 128) * (old scale / scale)) + 128,
+ * all in float32, ties to even. Writing the same tokens again changes nothing. x must be finite. */
+int qi_kv_append_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k,
+                    const void *v, int dtype, long long ld_k, long long ld_v, void *stream);
+
+/* The values that the cache holds for the batch's tokens, (code - 128) * scale, into k and v laid out as above. */
+int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, void *k, void *v,
+                  int dtype, long long ld_k, long long ld_v, void *stream);
+
+/* Attention of the batch's tokens over all tokens of their sequences in layer `layer`:
+ *   y[r, h] = sum_j softmax_j(scale * q[r, h] . k[j, h / (heads / kv_heads)]) v[j, h / (heads / kv_heads)]
+ * q and y [tokens, heads, head_dim] float16, ld_q and ld_y elements between rows (multiples of 8). Row i of an entry with
+ * c tokens of a sequence of n stands at position p = n - c + i. `causal`: it sees tokens j <= p; `window` > 0: it sees
+ * tokens j > p - window only. A row that sees nothing (no token, or p < 0) gives zeros. lse [tokens, heads] float32 or NULL
+ * receives log sum_j exp(scale * q . k), -infinity for such a row, with which results over several caches can be
+ * joined. Queries and weights enter the products as float16, codes exactly; all sums are float32. max_length bounds the
+ * lengths of the batch's sequences.
+ * workspace: qi_kv_attention_workspace() bytes (0: none needed) for the same cache, batch bounds, heads and max_length, 16-byte
+ * aligned, zeroed once before its first use; every call leaves its counters zero. One call at a time may use it. */
+typedef struct {
+    int layer, heads;
+    const void *q;
+    long long ld_q;
+    void *y;
+    long long ld_y;
+    float *lse;
+    float scale;
+    int causal, window, max_length;
+} qi_kv_attention;
+int qi_kv_attention_workspace(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, size_t *bytes);
+int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, const qi_kv_attention *call,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* Upkeep of the pages. Lists (slots, counts, parents, children, sources, targets) are device arrays of n int32. New pages are the
+ * lowest free ones, in the order of the list. workspace: qi_kv_pages_workspace() bytes, 16-byte aligned; nothing in it has to be
+ * cleared, and calls on one stream may share it. */
+int qi_kv_pages_workspace(const qi_kv_cache *cache, const qi_kv_pages *pages, size_t *bytes);
+
+/* Pages for counts[i] more tokens of sequence slots[i], whose length grows by them: for all of the list, or for none when too few
+ * pages are free. *shortage (device) becomes 0, how many pages are missing, or -1 where the list itself is at fault (an unknown
+ * sequence, or one too long for its row of the table). No sequence twice. */
+int qi_kv_pages_reserve_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *slots, const int *counts, int n,
+                           int *shortage, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Sequence children[i] becomes a copy of what sequence parents[i] was before the call (so a list may permute the beams of a search):
+ * whole pages are shared, the last one, if it is not full, is copied in every layer to a page of the child's own, taken from those that
+ * were free before the call. What a child held before is given back. child = parent changes nothing. No child twice. *shortage as
+ * above; nothing changes unless it is 0. */
+int qi_kv_pages_fork_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *parents, const int *children, int n,
+                        int *shortage, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The sequences end: their pages are given back, their lengths become 0, their rows of the table -1. No sequence twice. */
+int qi_kv_pages_free_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *slots, int n, void *stream);
+
+/* Moves the pages in use together at the front of the pool, in every layer, and renames them in the tables: the k-th page in use from
+ * *used on goes to the k-th free one before it. *used (device) becomes their number. */
+int qi_kv_pages_compact_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, int *used, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+/* Copies page sources[i] to page targets[i] in every layer, codes and scales. No page may be a target twice, or both source and target. */
+int qi_kv_pages_copy_ex(const qi_kv_cache *cache, const int *sources, const int *targets, int n, void *stream);
+
+/* The norms around a block, with the block's gate, in one pass over [rows, width]:
+ *   r' = residual + residual_scale * gate * post(branch)      post: norm * branch_weight if branch_norm, else * branch_weight
+ *   y  = norm(r') * weight * (1 + scale) + shift              norm: x / sqrt(mean(x^2) + epsilon), of x - mean(x) for QI_NORM_LAYER
+ * branch NULL: r' = residual. Weights [width] float32 or NULL (1). gate, scale, shift: vectors of `vector_dtype`, NULL (1, 0, 0), row r
+ * uses row r / rows_per_vector of each, ld_vector elements between rows, so that they may be columns of one modulation result.
+ * residual_out (residual_dtype, may be the residual itself) and y may be NULL, not both; y is none of the inputs. Sums are float32; y
+ * comes from r' before it is rounded to residual_dtype. width a multiple of 8, at most 16384; all pointers 16-byte aligned, ld_vector a
+ * multiple of 8. The reference's layer_norm_scale, rms_norm and gated_residual (qwen_image_cuda/cuda/ops.cu:37-118) are cases of it. */
+#define QI_NORM_LAYER 0
+#define QI_NORM_RMS 1
+typedef struct {
+    int rows, width, kind;
+    float epsilon;
+    const void *residual;
+    int residual_dtype;
+    const void *branch;
+    int branch_dtype, branch_norm;
+    const float *branch_weight;
+    float residual_scale;
+    const void *gate, *scale, *shift;
+    int vector_dtype;
+    long long ld_vector;
+    int rows_per_vector;
+    const float *weight;
+    void *residual_out, *y;
+    int y_dtype;
+} qi_gated_norm;
+int qi_gated_norm_ex(const qi_gated_norm *call, void *stream);
+
 /* ---- diagnostics --------------------------------------------------------------------------- */
 
 /* Kernels of this library never spin without a bound: a wait that runs out records a code

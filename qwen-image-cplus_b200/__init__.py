@@ -20,7 +20,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_HERE)
 LIB_PATH = os.path.join(_HERE, "libqipack_b200.so")
 SOURCES = ["qipack_b200.cu", "ptx.cuh", "quantize.cuh", "w4a16_gemm.cuh", "w4a16_gemv.cuh", "w4a16_gemv_stream.cuh", "w4a16_pair_gemm.cuh", "w4a16_swap_gemm.cuh", "w4a16_pair_swap_gemm.cuh", "w4a4_gemm.cuh",
-           "w4a4_wide_gemm.cuh", "w4a4_pair_gemm.cuh", "w4a4_narrow_gemm.cuh", "w4a4_tall_gemm.cuh", "shard.cuh", "probe.cuh", "pack_file.cuh"]
+           "w4a4_wide_gemm.cuh", "w4a4_pair_gemm.cuh", "w4a4_narrow_gemm.cuh", "w4a4_tall_gemm.cuh", "shard.cuh", "probe.cuh", "pack_file.cuh",
+           "kv_cache.cuh", "kv_pages.cuh", "kv_decode.cuh", "gated_norm.cuh", "block_ops.cuh"]
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -86,6 +87,37 @@ class qi_pack_tensor(ctypes.Structure):
                 ("zeros", ctypes.c_void_p), ("zeros_length", ctypes.c_uint64)]
 
 
+class qi_kv_cache(ctypes.Structure):
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("page_tokens", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int)]
+
+
+class qi_kv_pages(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("references", ctypes.c_void_p), ("sequences", ctypes.c_int),
+                ("table_pages", ctypes.c_int)]
+
+
+class qi_kv_batch(ctypes.Structure):
+    _fields_ = [("slots", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("entries", ctypes.c_int), ("tokens", ctypes.c_int),
+                ("most", ctypes.c_int)]
+
+
+class qi_kv_attention(ctypes.Structure):
+    _fields_ = [("layer", ctypes.c_int), ("heads", ctypes.c_int), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_longlong),
+                ("y", ctypes.c_void_p), ("ld_y", ctypes.c_longlong), ("lse", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("causal", ctypes.c_int), ("window", ctypes.c_int), ("max_length", ctypes.c_int)]
+
+
+class qi_gated_norm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int), ("width", ctypes.c_int), ("kind", ctypes.c_int), ("epsilon", ctypes.c_float),
+                ("residual", ctypes.c_void_p), ("residual_dtype", ctypes.c_int), ("branch", ctypes.c_void_p),
+                ("branch_dtype", ctypes.c_int), ("branch_norm", ctypes.c_int), ("branch_weight", ctypes.c_void_p),
+                ("residual_scale", ctypes.c_float), ("gate", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+                ("vector_dtype", ctypes.c_int), ("ld_vector", ctypes.c_longlong), ("rows_per_vector", ctypes.c_int),
+                ("weight", ctypes.c_void_p), ("residual_out", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_dtype", ctypes.c_int)]
+
+
 _P, _I, _LL, _ULL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong
 
 # name -> argument types; every entry point of include/qipack_b200.h
@@ -141,6 +173,18 @@ SIGNATURES = {
     "qi_pack_verify": [ctypes.c_char_p],
     "qi_pack_verify_ex": [ctypes.c_char_p, _I, _I],
     "qi_pack_write": [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(qi_pack_tensor), _I],
+    "qi_kv_append_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), ctypes.POINTER(qi_kv_batch), _I, _P, _P, _I, _LL, _LL, _P],
+    "qi_kv_read_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), ctypes.POINTER(qi_kv_batch), _I, _P, _P, _I, _LL, _LL, _P],
+    "qi_kv_attention_workspace": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_batch), _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "qi_kv_attention_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), ctypes.POINTER(qi_kv_batch),
+                           ctypes.POINTER(qi_kv_attention), _P, ctypes.c_size_t, _P],
+    "qi_kv_pages_workspace": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), ctypes.POINTER(ctypes.c_size_t)],
+    "qi_kv_pages_reserve_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), _P, _P, _I, _P, _P, ctypes.c_size_t, _P],
+    "qi_kv_pages_fork_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), _P, _P, _I, _P, _P, ctypes.c_size_t, _P],
+    "qi_kv_pages_free_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), _P, _I, _P],
+    "qi_kv_pages_compact_ex": [ctypes.POINTER(qi_kv_cache), ctypes.POINTER(qi_kv_pages), _P, _P, ctypes.c_size_t, _P],
+    "qi_kv_pages_copy_ex": [ctypes.POINTER(qi_kv_cache), _P, _P, _I, _P],
+    "qi_gated_norm_ex": [ctypes.POINTER(qi_gated_norm), _P],
     "qi_kernel_status": [ctypes.POINTER(ctypes.c_uint)],
     "qi_probe_tensor_rate": [_I, ctypes.c_double, ctypes.POINTER(ctypes.c_double)],
     "qi_probe_wait_timeout": [_ULL, _P],
@@ -393,6 +437,123 @@ def linear(model: PackedLinear, work: LinearWork, input, output, rows: int, reus
     return lib().qi_linear(ctypes.byref(model.record), ctypes.byref(work.work), _p(input), input_dtype, _p(output),
                            output_dtype, model.n if ld_output is None else ld_output, rows, int(reuse_input),
                            _p(stream))
+
+
+# ---- between the linears: norms, the 8-bit cache of keys and values, attention, pages (include/qipack_b200.h) ----
+
+NORM_LAYER, NORM_RMS = 0, 1
+KV_BLOCK = 16  # tokens that share a scale
+
+
+class KvCache:
+    """The pool: codes uint8 [layers, pages, kv_heads, page_tokens, head_dim], scales float32 [layers, pages, kv_heads, page_tokens / 16]."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales  # keep tensors alive
+        layers, pages, kv_heads, page_tokens, head_dim = k_codes.shape
+        if tuple(v_codes.shape) != tuple(k_codes.shape) or any(tuple(s.shape) != (layers, pages, kv_heads, page_tokens // KV_BLOCK) for s in (k_scales, v_scales)):
+            raise ValueError("the codes and scales of a cache do not belong together")
+        if not all(t.is_contiguous() for t in (k_codes, v_codes, k_scales, v_scales)):
+            raise ValueError("the codes and scales of a cache are contiguous")
+        self.cache = qi_kv_cache(_p(k_codes), _p(v_codes), _p(k_scales), _p(v_scales), layers, pages, page_tokens, kv_heads, head_dim)
+
+
+class KvPages:
+    """Which pages hold which tokens: table int32 [sequences, table_pages], lengths [sequences], references [pages]."""
+
+    def __init__(self, table, lengths, references):
+        self.table, self.lengths, self.references = table, lengths, references
+        sequences, table_pages = table.shape
+        if lengths.numel() != sequences or not all(t.is_contiguous() for t in (table, lengths, references)):
+            raise ValueError("a table of pages, its lengths and its references are contiguous and belong together")
+        self.pages = qi_kv_pages(_p(table), _p(lengths), _p(references), sequences, table_pages)
+
+
+class KvBatch:
+    """The last offsets[b + 1] - offsets[b] tokens of sequence slots[b] (None: b) for each entry; `tokens` rows, at most `most` for one."""
+
+    def __init__(self, slots, offsets, tokens: int, most: int):
+        self.slots, self.offsets = slots, offsets
+        self.batch = qi_kv_batch(_p(slots), _p(offsets), offsets.numel() - 1, tokens, most)
+
+
+def kv_append_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
+    """Quantises the batch's keys and values into their pages."""
+    return lib().qi_kv_append_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), layer, _p(k), _p(v), dtype, ld_k, ld_v, _p(stream))
+
+
+def kv_read_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
+    """The values that the cache holds for the batch's tokens."""
+    return lib().qi_kv_read_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), layer, _p(k), _p(v), dtype, ld_k, ld_v, _p(stream))
+
+
+def _bytes_of(workspace) -> int:
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def kv_attention_workspace(cache: KvCache, batch: KvBatch, heads: int, max_length: int) -> int:
+    """Bytes of workspace (to be zeroed once) that kv_attention_ex needs for batches within these bounds."""
+    value = ctypes.c_size_t(0)
+    status = lib().qi_kv_attention_workspace(ctypes.byref(cache.cache), ctypes.byref(batch.batch), heads, max_length, ctypes.byref(value))
+    if status != 0:
+        raise ValueError(f"no attention of {heads} heads over such a cache (status {status})")
+    return value.value
+
+
+def kv_attention_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, q, ld_q: int, y, ld_y: int, heads: int, scale: float, max_length: int, *,
+                    causal: bool = True, window: int = 0, lse=None, workspace=None, stream=None) -> int:
+    """y = attention of float16 q over the batch's sequences; lse float32 [tokens, heads] or None."""
+    call = qi_kv_attention(layer, heads, _p(q), ld_q, _p(y), ld_y, _p(lse), scale, int(causal), window, max_length)
+    return lib().qi_kv_attention_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), ctypes.byref(call), _p(workspace), _bytes_of(workspace), _p(stream))
+
+
+def kv_pages_workspace(cache: KvCache, pages: KvPages) -> int:
+    """Bytes of workspace of the calls below."""
+    value = ctypes.c_size_t(0)
+    status = lib().qi_kv_pages_workspace(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(value))
+    if status != 0:
+        raise ValueError(f"no such cache (status {status})")
+    return value.value
+
+
+def kv_pages_reserve_ex(cache: KvCache, pages: KvPages, slots, counts, count: int, shortage, workspace, stream=None) -> int:
+    """Pages for counts[i] more tokens of sequence slots[i]; `shortage` (device int32): 0, or how many pages are missing."""
+    return lib().qi_kv_pages_reserve_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(slots), _p(counts), count, _p(shortage), _p(workspace), _bytes_of(workspace), _p(stream))
+
+
+def kv_pages_fork_ex(cache: KvCache, pages: KvPages, parents, children, count: int, shortage, workspace, stream=None) -> int:
+    """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call."""
+    return lib().qi_kv_pages_fork_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(parents), _p(children), count, _p(shortage), _p(workspace), _bytes_of(workspace), _p(stream))
+
+
+def kv_pages_free_ex(cache: KvCache, pages: KvPages, slots, count: int, stream=None) -> int:
+    """The sequences end and give their pages back."""
+    return lib().qi_kv_pages_free_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(slots), count, _p(stream))
+
+
+def kv_pages_compact_ex(cache: KvCache, pages: KvPages, used, workspace, stream=None) -> int:
+    """Moves the pages in use together at the front; `used` (device int32) becomes their number."""
+    return lib().qi_kv_pages_compact_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(used), _p(workspace), _bytes_of(workspace), _p(stream))
+
+
+def kv_pages_copy_ex(cache: KvCache, sources, targets, count: int, stream=None) -> int:
+    """Copies page sources[i] to page targets[i] in every layer."""
+    return lib().qi_kv_pages_copy_ex(ctypes.byref(cache.cache), _p(sources), _p(targets), count, _p(stream))
+
+
+class GatedNorm:
+    """One call of gated_norm_ex: r' = residual + residual_scale * gate * post(branch), y = norm(r') * weight * (1 + scale) + shift."""
+
+    def __init__(self, rows: int, width: int, *, kind: int = NORM_LAYER, epsilon: float = 1e-6, residual, residual_dtype: int = DTYPE_F32, branch=None,
+                 branch_dtype: int = DTYPE_F32, branch_norm: bool = False, branch_weight=None, residual_scale: float = 1.0, gate=None, scale=None, shift=None,
+                 vector_dtype: int = DTYPE_F32, ld_vector: int = 0, rows_per_vector: int = 0, weight=None, residual_out=None, y=None, y_dtype: int = DTYPE_F32):
+        self.keep = (residual, branch, branch_weight, gate, scale, shift, weight, residual_out, y)
+        self.call = qi_gated_norm(rows, width, kind, epsilon, _p(residual), residual_dtype, _p(branch), branch_dtype, int(branch_norm), _p(branch_weight), residual_scale, _p(gate),
+                                  _p(scale), _p(shift), vector_dtype, ld_vector, rows_per_vector, _p(weight), _p(residual_out), _p(y), y_dtype)
+
+
+def gated_norm_ex(call: GatedNorm, stream=None) -> int:
+    return lib().qi_gated_norm_ex(ctypes.byref(call.call), _p(stream))
 
 
 # ---- the QIPACK v6 container (host side; int4_pack.cplus:36-95, 476-518, 733-850) ------------------------

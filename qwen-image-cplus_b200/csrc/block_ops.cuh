@@ -1,0 +1,288 @@
+// C ABI of the operators between the packed linears (include/qipack_b200.h): the norms around a block, the paged 8-bit cache, the
+// attention over it and the upkeep of its pages. Argument checks, plans and launches.
+#pragma once
+#include <algorithm>
+
+#include "gated_norm.cuh"
+#include "kv_cache.cuh"
+#include "kv_decode.cuh"
+#include "kv_pages.cuh"
+
+namespace qi {
+namespace {
+
+// SMs of the current device; where there is none, as many as a B200 has: plans need no device, and a launch then says what is missing.
+int sms_or_usual() {
+    const int device = current_device();
+    return device < 0 ? 148 : sm_count(device);
+}
+
+bool aligned4(const void *pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 3) == 0; }
+bool known_dtype(int dtype) { return dtype == QI_DTYPE_F32 || dtype == QI_DTYPE_F16; }
+
+// ---- the cache --------------------------------------------------------------------------------------------------------
+
+int page_shift_of(int page_tokens) {
+    for (int shift = 4; shift <= 8; ++shift)
+        if (page_tokens == 1 << shift) return shift;
+    return -1;
+}
+
+bool sound(const qi_kv_cache *cache) {
+    return cache && cache->k_codes && cache->v_codes && cache->k_scales && cache->v_scales && aligned16(cache->k_codes) && aligned16(cache->v_codes) &&
+           aligned4(cache->k_scales) && aligned4(cache->v_scales) && cache->layers > 0 && cache->pages > 0 && cache->kv_heads > 0 &&
+           cache->kv_heads <= 4096 && (cache->head_dim == 64 || cache->head_dim == 128) && page_shift_of(cache->page_tokens) > 0;
+}
+bool sound(const qi_kv_pages *pages) {
+    return pages && pages->table && pages->lengths && pages->references && aligned4(pages->table) && aligned4(pages->lengths) && aligned4(pages->references) &&
+           pages->sequences > 0 && pages->table_pages > 0 && pages->table_pages <= kv::MOST_TABLE_PAGES;
+}
+bool sound(const qi_kv_batch *batch) {
+    return batch && batch->offsets && aligned4(batch->offsets) && aligned4(batch->slots) && batch->entries >= 0 && batch->entries <= 65535 && batch->tokens >= 0 && batch->most >= 0;
+}
+
+kv::Cache layer_of(const qi_kv_cache *cache, int layer) {
+    kv::Cache c;
+    c.codes[0] = static_cast<uint8_t *>(cache->k_codes), c.codes[1] = static_cast<uint8_t *>(cache->v_codes);
+    c.scales[0] = cache->k_scales, c.scales[1] = cache->v_scales;
+    c.first_page = static_cast<long long>(layer) * cache->pages;
+    c.pages = cache->pages, c.heads = cache->kv_heads, c.page_shift = page_shift_of(cache->page_tokens);
+    return c;
+}
+kv::Tables tables_of(const qi_kv_pages *pages) { return {pages->table, pages->lengths, pages->references, pages->sequences, pages->table_pages}; }
+kv::Batch batch_of(const qi_kv_batch *batch) { return {batch->slots, batch->offsets, batch->entries, batch->tokens, batch->most}; }
+
+// A launch of any grid, overlapped with the kernel before it.
+template <typename... Parameters, typename... Arguments>
+int launch_grid(void (*kernel)(Parameters...), dim3 grid, int threads, int smem_bytes, void *stream, const Arguments &...arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem_bytes;
+    config.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return static_cast<int>(launched(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...)));
+}
+
+template <typename T>
+int launch_append(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k, const void *v, long long ld_k, long long ld_v, void *stream) {
+    const long long blocks = (static_cast<long long>(batch->most) + 2 * kv::BLOCK - 2) / kv::BLOCK;  // that `most` tokens in a row can touch
+    const long long units = blocks * cache->kv_heads * 2;
+    const long long grid = (units + kv::APPEND_WARPS - 1) / kv::APPEND_WARPS;
+    if (grid > 0x7fffffff / kv::APPEND_WARPS) return INVALID;
+    auto kernel = cache->head_dim == 128 ? kv::append_kernel<T, 128> : kv::append_kernel<T, 64>;
+    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::APPEND_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
+                       static_cast<const T *>(k), static_cast<const T *>(v), ld_k, ld_v);
+}
+
+template <typename T>
+int launch_read(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, void *k, void *v, long long ld_k, long long ld_v, void *stream) {
+    const long long quads = static_cast<long long>(batch->most) * cache->kv_heads * (cache->head_dim / 4), each = kv::READ_THREADS * kv::READ_ROWS;
+    const long long grid = (quads + each - 1) / each;
+    if (grid > 0x7fffffff) return INVALID;
+    auto kernel = cache->head_dim == 128 ? kv::read_kernel<T, 128> : kv::read_kernel<T, 64>;
+    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries, 2), kv::READ_THREADS, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
+                       static_cast<T *>(k), static_cast<T *>(v), ld_k, ld_v);
+}
+
+// ---- attention ----------------------------------------------------------------------------------------------------------
+
+struct AttentionPlan {
+    int tiles, rows, row_tiles, chunk, splits;
+    size_t partial_offset, bytes;
+};
+
+// How a call is cut: query rows into tiles, and the tokens of a tile into pieces where there are too few tiles for the GPU.
+bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int window, int sms, AttentionPlan &plan) {
+    if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
+    const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads);
+    plan.tiles = rows <= 8 ? 1 : 2;
+    plan.rows = 8 * plan.tiles;
+    const long long row_tiles = rows > 0 ? (rows + plan.rows - 1) / plan.rows : 1;
+    if (row_tiles * cache->kv_heads > 65535) return false;
+    plan.row_tiles = static_cast<int>(row_tiles);
+    const long long units = row_tiles * cache->kv_heads * (batch->entries > 0 ? batch->entries : 1);
+    long long span = max_length;  // of the tokens that a tile can see
+    if (window > 0 && static_cast<long long>(window) + batch->most + kv::BLOCK < span) span = static_cast<long long>(window) + batch->most + kv::BLOCK;
+    const long long round = kv::DECODE_WARPS * kv::STEP, wanted = 12LL * sms;
+    long long chunk = (span * units + wanted - 1) / wanted;
+    chunk = (chunk + round - 1) / round * round;
+    if (chunk < round) chunk = round;
+    long long splits = span > 0 ? (span + chunk - 1) / chunk : 1;
+    plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(splits);
+    plan.partial_offset = (static_cast<size_t>(units) * 4 + 255) / 256 * 256;
+    // room for as many pieces as any window gives
+    const long long most = std::min((wanted + units - 1) / units, (max_length + round - 1) / round);
+    plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * plan.rows * (cache->head_dim + 2) * 4 : 0;
+    return true;
+}
+
+kv::PageTables page_tables_of(const qi_kv_cache *cache, const qi_kv_pages *pages) {
+    return {pages->table, pages->lengths, pages->references, pages->sequences, pages->table_pages, cache->pages, page_shift_of(cache->page_tokens)};
+}
+
+size_t page_work_bytes(const qi_kv_cache *cache, const qi_kv_pages *pages) {
+    const size_t lists = static_cast<size_t>(cache->pages > pages->sequences ? cache->pages : pages->sequences);
+    return 4 * (4 + 2 * lists + cache->pages + static_cast<size_t>(pages->sequences) * pages->table_pages + pages->sequences);
+}
+
+kv::PageWork page_work_of(const qi_kv_cache *cache, const qi_kv_pages *pages, void *workspace) {
+    const size_t lists = static_cast<size_t>(cache->pages > pages->sequences ? cache->pages : pages->sequences);
+    kv::PageWork work;
+    work.count = static_cast<int *>(workspace);
+    work.sources = work.count + 4;
+    work.targets = work.sources + lists;
+    work.moved = work.targets + lists;
+    work.rows = work.moved + cache->pages;
+    work.held = work.rows + static_cast<size_t>(pages->sequences) * pages->table_pages;
+    return work;
+}
+
+int launch_copies(const qi_kv_cache *cache, const kv::PageTables &tables, const int *count, long long fixed_count, const int *sources, const int *targets, const int *moved, void *stream) {
+    kv::Pool pool;
+    pool.codes[0] = static_cast<uint8_t *>(cache->k_codes), pool.codes[1] = static_cast<uint8_t *>(cache->v_codes);
+    pool.scales[0] = cache->k_scales, pool.scales[1] = cache->v_scales;
+    pool.pages = cache->pages, pool.layers = cache->layers;
+    pool.page_bytes = cache->kv_heads * cache->page_tokens * cache->head_dim;
+    pool.page_scales = cache->kv_heads * (cache->page_tokens / kv::BLOCK);
+    return launch_grid(kv::copy_kernel, dim3(sms_or_usual() * 8), kv::COPY_THREADS, 0, stream, pool, count, static_cast<int>(fixed_count), sources, targets, tables, moved);
+}
+
+}  // namespace
+}  // namespace qi
+
+using namespace qi;
+
+extern "C" {
+
+int qi_kv_append_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k, const void *v, int dtype, long long ld_k, long long ld_v,
+                    void *stream) {
+    if (!sound(cache) || !sound(pages) || !sound(batch) || layer < 0 || layer >= cache->layers || !known_dtype(dtype)) return INVALID;
+    const long long width = static_cast<long long>(cache->kv_heads) * cache->head_dim, step = dtype == QI_DTYPE_F16 ? 8 : 4;
+    if (!k || !v || !aligned16(k) || !aligned16(v) || ld_k < width || ld_v < width || ld_k % step != 0 || ld_v % step != 0) return INVALID;
+    if (batch->entries == 0 || batch->most == 0) return 0;
+    return dtype == QI_DTYPE_F16 ? launch_append<__half>(cache, pages, batch, layer, k, v, ld_k, ld_v, stream) : launch_append<float>(cache, pages, batch, layer, k, v, ld_k, ld_v, stream);
+}
+
+int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, void *k, void *v, int dtype, long long ld_k, long long ld_v, void *stream) {
+    if (!sound(cache) || !sound(pages) || !sound(batch) || layer < 0 || layer >= cache->layers || !known_dtype(dtype)) return INVALID;
+    const long long width = static_cast<long long>(cache->kv_heads) * cache->head_dim, step = dtype == QI_DTYPE_F16 ? 8 : 4;
+    if (!k || !v || !aligned16(k) || !aligned16(v) || ld_k < width || ld_v < width || ld_k % step != 0 || ld_v % step != 0) return INVALID;
+    if (batch->entries == 0 || batch->most == 0) return 0;
+    return dtype == QI_DTYPE_F16 ? launch_read<__half>(cache, pages, batch, layer, k, v, ld_k, ld_v, stream) : launch_read<float>(cache, pages, batch, layer, k, v, ld_k, ld_v, stream);
+}
+
+int qi_kv_attention_workspace(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, size_t *bytes) {
+    AttentionPlan plan;
+    if (!sound(cache) || !sound(batch) || !bytes || !plan_attention(cache, batch, heads, max_length, 0, sms_or_usual(), plan)) return INVALID;
+    *bytes = plan.bytes;
+    return 0;
+}
+
+int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, const qi_kv_attention *call, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!sound(cache) || !sound(pages) || !sound(batch) || !call || call->layer < 0 || call->layer >= cache->layers) return INVALID;
+    if (call->heads <= 0 || call->heads % cache->kv_heads != 0 || call->heads > (1 << 20) / cache->head_dim) return INVALID;
+    const long long width = static_cast<long long>(call->heads) * cache->head_dim;
+    if (!call->q || !call->y || !aligned16(call->q) || !aligned16(call->y) || !aligned4(call->lse) || call->ld_q < width || call->ld_y < width || call->ld_q % 8 != 0 ||
+        call->ld_y % 8 != 0 || !(call->scale > 0.0f) || !(call->scale < INFINITY))
+        return INVALID;
+    AttentionPlan plan;
+    if (!plan_attention(cache, batch, call->heads, call->max_length, call->window, sms_or_usual(), plan)) return INVALID;
+    if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes)) return INVALID;
+    if (batch->entries == 0 || batch->most == 0) return 0;
+    kv::Attention a;
+    a.q = static_cast<const __half *>(call->q), a.y = static_cast<__half *>(call->y), a.lse = call->lse;
+    a.ld_q = call->ld_q, a.ld_y = call->ld_y;
+    a.heads = call->heads, a.group = call->heads / cache->kv_heads;
+    a.scale_log2 = call->scale * 1.4426950408889634f;
+    a.causal = call->causal, a.window = call->window, a.max_length = call->max_length;
+    a.chunk = plan.chunk, a.splits = plan.splits, a.row_tiles = plan.row_tiles;
+    a.arrivals = static_cast<int *>(workspace);
+    a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.partial_offset);
+    auto kernel = cache->head_dim == 128 ? (plan.tiles == 1 ? kv::decode_kernel<128, 1> : kv::decode_kernel<128, 2>)
+                                         : (plan.tiles == 1 ? kv::decode_kernel<64, 1> : kv::decode_kernel<64, 2>);
+    return launch_grid(kernel, dim3(plan.splits, cache->kv_heads * plan.row_tiles, batch->entries), kv::DECODE_THREADS, 0, stream, layer_of(cache, call->layer), tables_of(pages),
+                       batch_of(batch), a);
+}
+
+int qi_kv_pages_workspace(const qi_kv_cache *cache, const qi_kv_pages *pages, size_t *bytes) {
+    if (!sound(cache) || !sound(pages) || !bytes) return INVALID;
+    *bytes = page_work_bytes(cache, pages);
+    return 0;
+}
+
+int qi_kv_pages_reserve_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *slots, const int *counts, int n, int *shortage, void *workspace, size_t workspace_bytes,
+                           void *stream) {
+    if (!sound(cache) || !sound(pages) || !slots || !counts || !shortage || !aligned4(slots) || !aligned4(counts) || !aligned4(shortage) || n < 0 || n > pages->sequences ||
+        !workspace || !aligned16(workspace) || workspace_bytes < page_work_bytes(cache, pages))
+        return INVALID;
+    return launch_grid(kv::reserve_kernel, dim3(1), kv::PLAN_THREADS, 0, stream, page_tables_of(cache, pages), slots, counts, n, shortage, page_work_of(cache, pages, workspace));
+}
+
+int qi_kv_pages_fork_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *parents, const int *children, int n, int *shortage, void *workspace, size_t workspace_bytes,
+                        void *stream) {
+    if (!sound(cache) || !sound(pages) || !parents || !children || !shortage || !aligned4(parents) || !aligned4(children) || !aligned4(shortage) || n < 0 || n > pages->sequences ||
+        !workspace || !aligned16(workspace) || workspace_bytes < page_work_bytes(cache, pages))
+        return INVALID;
+    const kv::PageTables tables = page_tables_of(cache, pages);
+    const kv::PageWork work = page_work_of(cache, pages, workspace);
+    const int status = launch_grid(kv::fork_kernel, dim3(1), kv::PLAN_THREADS, 0, stream, tables, parents, children, n, shortage, work);
+    return status != 0 ? status : launch_copies(cache, tables, work.count, 0, work.sources, work.targets, nullptr, stream);
+}
+
+int qi_kv_pages_free_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *slots, int n, void *stream) {
+    if (!sound(cache) || !sound(pages) || !slots || !aligned4(slots) || n < 0 || n > pages->sequences) return INVALID;
+    if (n == 0) return 0;
+    const int grid = (n + kv::PLAN_THREADS / 32 - 1) / (kv::PLAN_THREADS / 32);
+    return launch_grid(kv::free_kernel, dim3(grid), kv::PLAN_THREADS, 0, stream, page_tables_of(cache, pages), slots, n);
+}
+
+int qi_kv_pages_compact_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, int *used, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!sound(cache) || !sound(pages) || !used || !aligned4(used) || !workspace || !aligned16(workspace) || workspace_bytes < page_work_bytes(cache, pages)) return INVALID;
+    const kv::PageTables tables = page_tables_of(cache, pages);
+    const kv::PageWork work = page_work_of(cache, pages, workspace);
+    const int status = launch_grid(kv::compact_kernel, dim3(1), kv::PLAN_THREADS, 0, stream, tables, used, work);
+    return status != 0 ? status : launch_copies(cache, tables, work.count, 0, work.sources, work.targets, work.moved, stream);
+}
+
+int qi_kv_pages_copy_ex(const qi_kv_cache *cache, const int *sources, const int *targets, int n, void *stream) {
+    if (!sound(cache) || !sources || !targets || !aligned4(sources) || !aligned4(targets) || n < 0 || n > cache->pages) return INVALID;
+    if (n == 0) return 0;
+    return launch_copies(cache, kv::PageTables{}, nullptr, n, sources, targets, nullptr, stream);
+}
+
+int qi_gated_norm_ex(const qi_gated_norm *call, void *stream) {
+    if (!call || call->rows < 0 || call->width <= 0 || call->width > gated_norm::MOST_WIDTH || call->width % 8 != 0) return INVALID;
+    if (call->kind != QI_NORM_LAYER && call->kind != QI_NORM_RMS) return INVALID;
+    if (!known_dtype(call->residual_dtype) || !known_dtype(call->branch_dtype) || !known_dtype(call->vector_dtype) || !known_dtype(call->y_dtype)) return INVALID;
+    if (!call->residual || (!call->y && !call->residual_out) || !(call->epsilon >= 0.0f) || !(call->epsilon < INFINITY)) return INVALID;
+    const void *pointers[] = {call->residual, call->branch, call->branch_weight, call->gate, call->scale, call->shift, call->weight, call->residual_out, call->y};
+    for (const void *pointer : pointers)
+        if (!aligned16(pointer)) return INVALID;
+    if (!call->branch && (call->branch_norm || call->branch_weight || call->gate)) return INVALID;  // nothing to apply them to
+    if (call->gate || call->scale || call->shift)
+        if (call->rows_per_vector <= 0 || call->ld_vector < call->width || call->ld_vector % 8 != 0) return INVALID;
+    if (call->rows == 0) return 0;
+    gated_norm::Arguments a;
+    a.residual = call->residual, a.branch = call->branch, a.branch_weight = call->branch_weight;
+    a.gate = call->gate, a.scale = call->scale, a.shift = call->shift, a.weight = call->weight;
+    a.residual_out = call->residual_out, a.y = call->y;
+    a.ld_vector = call->ld_vector, a.rows = call->rows, a.width = call->width;
+    a.rows_per_vector = call->rows_per_vector > 0 ? call->rows_per_vector : call->rows;
+    a.residual_scale = call->residual_scale, a.epsilon = call->epsilon;
+    a.residual_f16 = call->residual_dtype == QI_DTYPE_F16, a.branch_f16 = call->branch_dtype == QI_DTYPE_F16;
+    a.vector_f16 = call->vector_dtype == QI_DTYPE_F16, a.y_f16 = call->y_dtype == QI_DTYPE_F16;
+    a.branch_norm = call->branch_norm != 0, a.layer = call->kind == QI_NORM_LAYER;
+    const int most = sms_or_usual() * 8, grid = a.rows < most ? a.rows : most;
+    if (a.width <= 1024) return launch_grid(gated_norm::norm_kernel<128, 1>, dim3(grid), 128, 0, stream, a);
+    if (a.width <= 2048) return launch_grid(gated_norm::norm_kernel<256, 1>, dim3(grid), 256, 0, stream, a);
+    if (a.width <= 4096) return launch_grid(gated_norm::norm_kernel<256, 2>, dim3(grid), 256, 0, stream, a);
+    if (a.width <= 8192) return launch_grid(gated_norm::norm_kernel<512, 2>, dim3(grid), 512, 0, stream, a);
+    return launch_grid(gated_norm::norm_kernel<512, 4>, dim3(grid), 512, 0, stream, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,183 @@
+// The norms on both sides of a block with the block's gate, in one pass over the rows:
+//
+//   r' = r + residual_scale * gate * post(branch)          post: a norm of the block's result times its weight, or nothing
+//   y  = norm(r') * weight * (1 + scale) + shift           norm: x / rms(x), or (x - mean) / deviation
+//
+// Each row is read once and written once; the values stay in registers between the sums, which are float32 and taken about the
+// mean (two passes over registers, so that a large mean costs no digits). r' enters the second norm unrounded, also where it is
+// stored as float16. Bound by memory: THREADS threads hold a row, 8 adjacent values a piece, so that every access is 16 bytes a thread or
+// more. CTAs walk over rows; the vectors (gate, scale, shift, weights) then come from L1, past which the rows are streamed.
+#pragma once
+#include "ptx.cuh"
+
+namespace qi {
+namespace gated_norm {
+
+constexpr int MOST_WIDTH = 16384;
+
+struct Arguments {
+    const void *residual, *branch;
+    const float *branch_weight;
+    const void *gate, *scale, *shift;
+    const float *weight;
+    void *residual_out, *y;
+    long long ld_vector;
+    int rows, width, rows_per_vector;
+    float residual_scale, epsilon;
+    bool residual_f16, branch_f16, vector_f16, y_f16, branch_norm, layer;
+};
+
+__device__ __forceinline__ void widen8(const uint4 w, float (&x)[8]) {
+    const uint32_t pairs[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[j]));
+        x[2 * j] = f.x, x[2 * j + 1] = f.y;
+    }
+}
+
+// Eight values from `at` on: a row's, which are read once (STREAM), or a vector's, which other rows read too.
+template <bool STREAM>
+__device__ __forceinline__ void load8(const void *base, bool f16, long long at, float (&x)[8]) {
+    if (f16) {
+        const uint4 *words = reinterpret_cast<const uint4 *>(static_cast<const __half *>(base) + at);
+        widen8(STREAM ? __ldcs(words) : __ldg(words), x);
+    } else {
+        const float4 *words = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+        const float4 a = STREAM ? __ldcs(words) : __ldg(words), b = STREAM ? __ldcs(words + 1) : __ldg(words + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    }
+}
+
+__device__ __forceinline__ void store8(void *base, bool f16, long long at, const float (&x)[8]) {
+    if (f16) {
+        uint32_t pairs[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+            pairs[j] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        *reinterpret_cast<uint4 *>(static_cast<__half *>(base) + at) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+    } else {
+        float4 *words = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
+        words[0] = make_float4(x[0], x[1], x[2], x[3]);
+        words[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+// Sum over the CTA. Two rows of `sums` in turn: a thread that writes the next sum's has passed the barrier behind which all have
+// read the one before the last.
+template <int WARPS>
+__device__ __forceinline__ float block_sum(float value, float (&sums)[2][WARPS], int &turn) {
+#pragma unroll
+    for (int step = 16; step > 0; step /= 2) value += __shfl_xor_sync(0xffffffffu, value, step);
+    if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = value;
+    __syncthreads();
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += sums[turn][w];
+    turn ^= 1;
+    return total;
+}
+
+template <int THREADS, int PIECES>
+__global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ float sums[2][WARPS];
+    grid_wait();
+    int turn = 0;
+    const float per_value = 1.0f / static_cast<float>(a.width);
+    // x becomes (x - mean if it is a layer norm) and its factor is returned
+    auto normalise = [&](float (&x)[PIECES][8]) {
+        if (a.layer) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += x[p][j];
+            const float mean = block_sum<WARPS>(sum, sums, turn) * per_value;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+                if ((p * THREADS + static_cast<int>(threadIdx.x)) * 8 < a.width)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[p][j] -= mean;
+        }
+        float squares = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) squares = fmaf(x[p][j], x[p][j], squares);
+        return rsqrtf(fmaf(block_sum<WARPS>(squares, sums, turn), per_value, a.epsilon));
+    };
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long long start = static_cast<long long>(row) * a.width, vector = static_cast<long long>(row / a.rows_per_vector) * a.ld_vector;
+        float r[PIECES][8], b[PIECES][8];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int column = (p * THREADS + threadIdx.x) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[p][j] = b[p][j] = 0.0f;
+            if (column < a.width) {
+                load8<true>(a.residual, a.residual_f16, start + column, r[p]);
+                if (a.branch != nullptr) load8<true>(a.branch, a.branch_f16, start + column, b[p]);
+            }
+        }
+        if (a.branch != nullptr) {
+            const float factor = a.branch_norm ? normalise(b) : 1.0f;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) {
+                const int column = (p * THREADS + threadIdx.x) * 8;
+                if (column >= a.width) continue;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[p][j] *= factor;
+                if (a.branch_weight != nullptr) {
+                    load8<false>(a.branch_weight, false, column, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
+                }
+                if (a.gate != nullptr) {
+                    load8<false>(a.gate, a.vector_f16, vector + column, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[p][j] = fmaf(a.residual_scale, b[p][j], r[p][j]);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int column = (p * THREADS + threadIdx.x) * 8;
+            if (column < a.width && a.residual_out != nullptr) store8(a.residual_out, a.residual_f16, start + column, r[p]);
+        }
+        if (a.y == nullptr) continue;
+        const float factor = normalise(r);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int column = (p * THREADS + threadIdx.x) * 8;
+            if (column >= a.width) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[p][j] *= factor;
+            if (a.weight != nullptr) {
+                load8<false>(a.weight, false, column, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[p][j] *= v[j];
+            }
+            if (a.scale != nullptr) {
+                load8<false>(a.scale, a.vector_f16, vector + column, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[p][j] *= 1.0f + v[j];
+            }
+            if (a.shift != nullptr) {
+                load8<false>(a.shift, a.vector_f16, vector + column, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[p][j] += v[j];
+            }
+            store8(a.y, a.y_f16, start + column, r[p]);
+        }
+    }
+}
+
+}  // namespace gated_norm
+}  // namespace qi

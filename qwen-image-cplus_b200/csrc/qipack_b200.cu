@@ -1196,5 +1196,6 @@ const char *qi_b200_version(void) { return "qipack_b200 0.1 sm_100a"; }
 
 }  // extern "C"
 
+#include "block_ops.cuh"
 #include "shard.cuh"
 #include "pack_file.cuh"

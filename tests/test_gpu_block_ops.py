@@ -1,0 +1,630 @@
+"""The operators between the packed linears through the C ABI, against plain implementations in 64 bits: the norms around a block, the
+paged 8-bit cache, the attention over it, the upkeep of its pages; and what they refuse."""
+import math
+import os
+import random
+
+import pytest
+
+import __graft_entry__ as entry
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+BLOCK = 16
+
+
+@pytest.fixture(scope="module")
+def qi():
+    if not torch.cuda.is_available():
+        pytest.fail("the gpu tests need a CUDA device")
+    module = entry.load_package()
+    if not os.path.exists(module.LIB_PATH):
+        module.build()
+    module.lib()
+    return module
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def settled(qi):
+    torch.cuda.synchronize()
+    assert qi.kernel_status() == 0
+
+
+class Store:
+    """A pool with sequences in scattered pages, and the values that it holds in 64 bits."""
+
+    def __init__(self, qi, seed, lengths, *, kv_heads=2, head_dim=128, page=32, layers=2, layer=1, spare=3, table_extra=0, fill=True):
+        self.qi, self.layer, self.page, self.kv_heads, self.head_dim, self.lengths_list = qi, layer, page, kv_heads, head_dim, lengths
+        rng = random.Random(seed)
+        needed = [-(-n // page) for n in lengths]
+        pages = max(sum(needed) + spare, 1)
+        order = list(range(pages))
+        rng.shuffle(order)
+        width = max(needed + [1]) + table_extra
+        references, table = [0] * pages, []
+        for n in needed:
+            mine = [order.pop() for _ in range(n)]
+            for p in mine:
+                references[p] = 1
+            table.append(mine + [-1] * (width - n))
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        shape, scales = (layers, pages, kv_heads, page, head_dim), (layers, pages, kv_heads, page // BLOCK)
+        self.codes, self.scales = {}, {}
+        for which in "kv":
+            if fill:
+                self.codes[which] = (torch.randn(*shape, device="cuda", generator=g) * 40 + 128).round().clamp(1, 255).to(torch.uint8)
+                self.scales[which] = torch.rand(*scales, device="cuda", generator=g) * 0.03 + 0.01
+            else:  # what a fresh allocation may hold
+                self.codes[which] = torch.randint(0, 256, shape, device="cuda", generator=g, dtype=torch.uint8)
+                self.scales[which] = torch.full(scales, float("nan"), device="cuda")
+        self.table, self.lengths, self.references = ints(table), ints(lengths), ints(references)
+        if fill:  # nothing may depend on scales of blocks that hold no token
+            for s, n in enumerate(lengths):
+                for block in range(-(-n // BLOCK), needed[s] * (page // BLOCK)):
+                    for which in "kv":
+                        self.scales[which][:, table[s][block * BLOCK // page], :, block % (page // BLOCK)] = float("nan")
+        self.cache = qi.KvCache(self.codes["k"], self.codes["v"], self.scales["k"], self.scales["v"])
+        self.pages = qi.KvPages(self.table, self.lengths, self.references)
+
+    def values(self, which, s, length=None):
+        """[tokens, kv_heads, head_dim] in 64 bits."""
+        length = self.lengths_list[s] if length is None else length
+        mine = self.table[s, : -(-length // self.page)].long()
+        codes = self.codes[which][self.layer, mine].transpose(1, 2).reshape(-1, self.kv_heads, self.head_dim)[:length].double() - 128
+        scales = self.scales[which][self.layer, mine].transpose(1, 2).reshape(-1, self.kv_heads)
+        return codes * scales.double().repeat_interleave(BLOCK, 0)[:length, :, None]
+
+    def batch(self, slots, counts, spare_tokens=0, most=None):
+        offsets = [sum(counts[:b]) for b in range(len(counts) + 1)]
+        return self.qi.KvBatch(ints(slots), ints(offsets), sum(counts) + spare_tokens, max(counts + [0]) if most is None else most)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+#
+# Tolerance. Codes, queries and products are exact; sums are float32. Weights p are rounded to float16 (relative 2^-11 at most, each by
+# itself), y to float16 (2^-11). An element of y is a weighted mean of values: |error| <= 2^-11 * sum p|v| / sum p + 2^-11 |y| + the float32
+# sums' part, which for 8192 terms in any order is below 2^-13 of the same mean. sum p|v| / sum p <= max |v|, so 2^-10 * max|v| bounds
+# every element, and the 2-norm, where the roundings are independent, is below 2^-11 of the result's. lse: 2^-21 * (|lse| + |x| max), x the
+# scores in base 2 (the fused multiply-add and ex2.approx, 2^-22 each), below 1e-5 absolute for scores below 16.
+
+
+def attend_exact(store, q, slots, counts, heads, scale, causal, window):
+    ys, lses, begin = [], [], 0
+    group = heads // store.kv_heads
+    for s, count in zip(slots, counts):
+        length = store.lengths_list[s]
+        k, v = (store.values(which, s).repeat_interleave(group, 1) for which in "kv")
+        mine = q[begin:begin + count].double()
+        begin += count
+        scores = torch.einsum("ihd,jhd->hij", mine, k) * scale
+        p, j = torch.arange(length - count, length, device="cuda")[:, None], torch.arange(length, device="cuda")[None]
+        hidden = torch.zeros(count, length, dtype=torch.bool, device="cuda")
+        if causal:
+            hidden |= j > p
+        if window:
+            hidden |= j <= p - window
+        scores = scores.masked_fill(hidden, -math.inf)
+        lse = torch.logsumexp(scores, 2) if length else torch.full((heads, count), -math.inf, dtype=torch.float64, device="cuda")
+        weights = torch.exp(scores - torch.where(lse == -math.inf, 0.0, lse)[..., None])
+        ys.append(torch.einsum("hij,jhd->ihd", weights, v))
+        lses.append(lse.T)
+    return torch.cat(ys), torch.cat(lses)
+
+
+def attend(qi, store, slots, counts, heads, *, causal=True, window=0, seed=1, gap=0, max_length=None, most=None, stream=None, q=None):
+    tokens, dim = sum(counts), store.head_dim
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if q is None:
+        q = (torch.randn(tokens, heads, dim, device="cuda", generator=g) * 1.5).half()
+    rows = torch.full((tokens, heads * dim + gap), float("nan"), dtype=torch.float16, device="cuda")
+    rows[:, : heads * dim] = q.view(tokens, -1)
+    y = torch.full((tokens, heads * dim + gap), float("nan"), dtype=torch.float16, device="cuda")
+    lse = torch.full((tokens, heads), float("nan"), device="cuda")
+    batch = store.batch(slots, counts, most=most)
+    max_length = max(store.lengths_list) if max_length is None else max_length
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, batch, heads, max_length), dtype=torch.uint8, device="cuda")
+    results = []
+    for _ in range(2):  # the second call finds the workspace as the first one left it
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream())
+        status = qi.kv_attention_ex(store.cache, store.pages, batch, store.layer, rows, heads * dim + gap, y, heads * dim + gap, heads, dim ** -0.5, max_length, causal=causal,
+                                    window=window, lse=lse, workspace=workspace, stream=None if stream is None else stream.cuda_stream)
+        assert status == 0
+        settled(qi)
+        results.append((y.clone(), lse.clone()))
+    assert torch.equal(results[0][0].view(torch.int16), results[1][0].view(torch.int16)) and torch.equal(results[0][1], results[1][1]), "two calls, two results"
+    assert gap == 0 or y[:, heads * dim:].isnan().all(), "written beyond the row"
+    got, exact, exact_lse = y[:, : heads * dim].view(tokens, heads, dim).double(), *attend_exact(store, q, slots, counts, heads, dim ** -0.5, causal, window)
+    assert torch.equal(lse == -math.inf, exact_lse == -math.inf)
+    seen = exact_lse > -math.inf
+    assert (got[~seen] == 0).all()
+    if seen.any():
+        largest = max(store.values("v", s).abs().max().item() for s in slots if store.lengths_list[s])
+        assert not got.isnan().any()
+        assert (got - exact).abs().max().item() <= 2.0 ** -10 * largest
+        assert (got - exact).norm().item() <= 2.0 ** -11 * exact.norm().item()
+        assert (lse.double() - exact_lse)[seen].abs().max().item() <= 1e-5
+    return y
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 127, 128, 129, 333, 1000])
+def test_one_token_of_one_sequence(qi, length, head_dim):
+    attend(qi, Store(qi, length, [length], head_dim=head_dim), [0], [1], 8)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_pages_of_every_size(qi, page):
+    store = Store(qi, page, [5, 300, 64, 17], page=page)
+    attend(qi, store, [2, 0, 3, 1], [1, 1, 1, 1], 2)
+    attend(qi, store, [1, 3], [211, 17], 2)
+
+
+@pytest.mark.parametrize("kv_heads,heads", [(1, 1), (1, 7), (3, 3), (2, 10), (4, 32), (1, 17), (5, 40)])
+@pytest.mark.parametrize("most", [1, 3, 40])
+def test_groups_of_heads(qi, kv_heads, heads, most):
+    store = Store(qi, heads, [most, 77, 150, 200], kv_heads=kv_heads, head_dim=64 if heads == 10 else 128)
+    attend(qi, store, [0, 1, 2, 3], [most, 1, most, min(most, 2)], heads)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("window", [0, 1, 15, 16, 100, 5000])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [5, 1, 8], [130, 300, 257]])
+def test_masks(qi, causal, window, counts):
+    attend(qi, Store(qi, window, [140, 650, 257]), [0, 1, 2], counts, 6, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("heads", [2, 16])
+def test_rows_that_see_nothing(qi, heads):
+    # sequences without a token, more queries than tokens, entries without a query
+    store = Store(qi, 7, [0, 3, 20, 40, 400])
+    attend(qi, store, [0, 1, 2, 3, 4], [1, 5, 0, 2, 1], heads)
+    attend(qi, store, [0, 1, 2, 4], [30, 200, 300, 0], heads)
+    attend(qi, store, [1, 0], [200, 4], heads, window=2)
+    attend(qi, store, [0, 4], [1, 3], heads, causal=False)
+
+
+def test_long_cache_is_split(qi):
+    store = Store(qi, 3, [20011, 1, 9000], page=64)
+    attend(qi, store, [0, 1, 2], [1, 1, 1], 8)
+    attend(qi, store, [0, 2], [4, 2], 8)
+    attend(qi, store, [0, 2], [150, 70], 8)
+    attend(qi, store, [0], [1], 8, max_length=64 * store.table.shape[1])
+
+
+def test_many_queries(qi):
+    store = Store(qi, 4, [1500, 1300, 129], page=64, kv_heads=2)
+    attend(qi, store, [0, 1, 2], [1500, 700, 129], 4)
+    attend(qi, store, [2, 1], [128, 1024], 2, causal=False)
+    attend(qi, store, [1], [999], 14, window=300)
+
+
+def test_strides_streams_and_loose_bounds(qi):
+    store = Store(qi, 5, [500, 300])
+    stream = torch.cuda.Stream()
+    for counts in ([1, 1], [200, 33]):
+        attend(qi, store, [1, 0], counts, 4, gap=24, stream=stream, max_length=900, most=max(counts) + 50)
+
+
+@pytest.mark.parametrize("count", [1, 200])
+def test_scales_that_differ_widely(qi, count):
+    store = Store(qi, 6, [700])
+    store.scales["v"][:, :, :, 0] *= 1000
+    store.scales["v"][:, 3] = 0.0
+    store.codes["v"][:, 3] = 128  # a page of zeros
+    store.scales["k"][:, 5] = 0.0
+    attend(qi, store, [0], [count], 4)
+    for which in "kv":  # a dominant key far from the end
+        store.codes[which][:, int(store.table[0, 2]), :, 5] = 255
+    attend(qi, store, [0], [count], 4)
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [100, 300]])
+def test_attention_in_a_graph_follows_lengths_on_the_device(qi, counts):
+    store = Store(qi, 8, [700, 640])
+    heads, dim = 4, 128
+    batch = store.batch([0, 1], counts)
+    q = torch.randn(sum(counts), heads, dim, device="cuda").half()
+    y = torch.zeros_like(q)
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, batch, heads, 700), dtype=torch.uint8, device="cuda")
+    call = lambda stream=None: qi.kv_attention_ex(store.cache, store.pages, batch, store.layer, q, heads * dim, y, heads * dim, heads, dim ** -0.5, 700, workspace=workspace, stream=stream)  # noqa: E731
+    assert call() == 0
+    settled(qi)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert call(torch.cuda.current_stream().cuda_stream) == 0
+    for lengths in ([700, 640], [650, 301], [400, 640]):
+        store.lengths.copy_(ints(lengths))
+        store.lengths_list = lengths
+        graph.replay()
+        settled(qi)
+        exact, _ = attend_exact(store, q, [0, 1], counts, heads, dim ** -0.5, True, 0)
+        assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm()
+
+
+# ---- append and read back ------------------------------------------------------------------------------------------
+#
+# Codes and scales are equal to the definition's in 32 bits, bit for bit: a division, a rounding and a product, each IEEE's.
+
+
+def append_plain(store, kv, slots, counts):
+    """The definition, block by block, on the CPU in float32."""
+    begin = 0
+    for s, count in zip(slots, counts):
+        length = store.lengths_list[s]
+        start = length - count
+        for block in range(start // BLOCK, -(-length // BLOCK) if count else 0):
+            first, end = max(start, block * BLOCK), min(length, (block + 1) * BLOCK)
+            page = int(store.table[s, block * BLOCK // store.page])
+            within = block * BLOCK % store.page
+            for which, x in kv.items():
+                new = x[begin + first - start:begin + end - start].float().cpu()
+                codes, scales = store.codes[which][store.layer, page].cpu(), store.scales[which][store.layer, page].cpu()
+                scale = new.abs().amax((0, 2)) / torch.tensor(127.0)
+                early = first - block * BLOCK
+                if early:
+                    old = scales[:, within // BLOCK]
+                    scale = torch.maximum(scale, old)
+                    factor = torch.where(scale > 0, old / scale, torch.ones(()))
+                    kept = codes[:, within:within + early].float() - 128
+                    codes[:, within:within + early] = ((kept * factor[:, None, None]).round() + 128).to(torch.uint8)
+                q = torch.where(scale[None, :, None] > 0, new / scale[None, :, None], torch.zeros(())).round().clamp(-127, 127) + 128
+                codes[:, within + early:within + early + len(new)] = q.to(torch.uint8).transpose(0, 1)
+                scales[:, within // BLOCK] = scale
+                store.codes[which][store.layer, page], store.scales[which][store.layer, page] = codes.cuda(), scales.cuda()
+        begin += count
+
+
+def same_bytes(a, b):
+    return all(torch.equal(a.codes[w], b.codes[w]) and torch.equal(a.scales[w].view(torch.int32), b.scales[w].view(torch.int32)) for w in "kv")
+
+
+def make_kv(store, tokens, dtype, seed, gap=0, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    width = store.kv_heads * store.head_dim
+    rows = torch.randn(tokens, 2 * width + gap, device="cuda", generator=g) * torch.exp2(torch.randn(tokens, 1, device="cuda", generator=g) * spread)
+    rows = rows.to(dtype)
+    return rows, {"k": rows[:, :width].view(tokens, -1, store.head_dim) if tokens else rows, "v": rows[:, width:2 * width].reshape(tokens, -1, store.head_dim) if tokens else rows}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("head_dim,page,kv_heads", [(128, 32, 2), (64, 16, 3), (128, 256, 1), (64, 64, 5)])
+def test_append_equals_the_definition_and_reads_back(qi, dtype, head_dim, page, kv_heads):
+    lengths, counts, slots = [1, 16, 17, 100, 333, 64, 5], [1, 16, 1, 33, 300, 0, 3], [0, 1, 2, 3, 4, 5, 6]
+    code = qi.DTYPE_F16 if dtype == torch.float16 else qi.DTYPE_F32
+    a, b = (Store(qi, 11, lengths, kv_heads=kv_heads, head_dim=head_dim, page=page) for _ in range(2))
+    rows, kv = make_kv(a, sum(counts), dtype, 12, gap=16)
+    width, ld = kv_heads * head_dim, 2 * kv_heads * head_dim + 16
+    append_plain(b, kv, slots, counts)
+    for _ in range(2):  # writing the same tokens again changes nothing
+        assert qi.kv_append_ex(a.cache, a.pages, a.batch(slots, counts), 1, rows, rows[:, width:], code, ld, ld) == 0
+        settled(qi)
+        assert same_bytes(a, b)
+    out = torch.full((2, sum(counts), width + 8), float("nan"), dtype=dtype, device="cuda")
+    assert qi.kv_read_ex(a.cache, a.pages, a.batch(slots, counts), 1, out[0], out[1], code, width + 8, width + 8) == 0
+    settled(qi)
+    assert out[:, :, width:].isnan().all()
+    for i, which in enumerate("kv"):
+        # one product in float32, rounded once more where the result is float16
+        expected = torch.cat([a.values(which, s)[len(a.values(which, s)) - n:] for s, n in zip(slots, counts)]).float().to(dtype)
+        assert torch.equal(out[i, :, :width].view(expected.shape), expected)
+
+
+def test_append_token_by_token_into_fresh_pages(qi):
+    # pages as an allocation leaves them: scales NaN, any codes. Scales only grow within a block, earlier tokens are rounded again.
+    steps = 37
+    a, b = (Store(qi, 13, [steps], page=16, fill=False) for _ in range(2))
+    rows, kv = make_kv(a, steps, torch.float32, 14, spread=2.0)
+    width = a.kv_heads * a.head_dim
+    for t in range(1, steps + 1):
+        for store in (a, b):
+            store.lengths_list = [t]
+            store.lengths.copy_(ints([t]))
+        append_plain(b, {w: x[t - 1:t] for w, x in kv.items()}, [0], [1])
+        assert qi.kv_append_ex(a.cache, a.pages, a.batch([0], [1]), 1, rows[t - 1:], rows[t - 1:, width:], qi.DTYPE_F32, 2 * width, 2 * width) == 0
+    settled(qi)
+    assert same_bytes(a, b)
+    # the values are as near as codes of that scale can be: half a step from the last rounding, and half a step of each scale before it (at
+    # most 15 times, each step no wider than the last one)
+    held = a.values("k", 0)
+    step = a.scales["k"][1].nan_to_num(0.0).max().double()  # the spare pages hold no token
+    assert (held - kv["k"].double()).abs().max() <= 8 * step
+
+
+def test_append_of_zeros_and_of_extremes(qi):
+    store, plain = (Store(qi, 15, [16, 32], fill=False) for _ in range(2))
+    rows, _ = make_kv(store, 48, torch.float32, 16)
+    width = store.kv_heads * store.head_dim
+    rows[:16] = 0.0
+    rows[16:24] *= 1e30
+    rows[24:32] *= 1e-30
+    kv = {"k": rows[:, :width].view(48, -1, store.head_dim), "v": rows[:, width:].reshape(48, -1, store.head_dim)}
+    append_plain(plain, kv, [0, 1], [16, 32])
+    assert qi.kv_append_ex(store.cache, store.pages, store.batch([0, 1], [16, 32]), 1, rows, rows[:, width:], qi.DTYPE_F32, 2 * width, 2 * width) == 0
+    settled(qi)
+    assert same_bytes(store, plain)
+    y = torch.zeros(1, 2, 128, dtype=torch.float16, device="cuda")
+    assert qi.kv_attention_ex(store.cache, store.pages, store.batch([0], [1]), 1, torch.ones_like(y), 256, y, 256, 2, 1.0, 16) == 0
+    settled(qi)
+    assert (y == 0).all()
+
+
+def test_append_leaves_shared_and_missing_pages_alone(qi):
+    # page numbers are the device's own: what must not be written is left as it is, and the status word says so
+    for fault in ("shared", "missing", "foreign", "count", "slot"):
+        store, before = (Store(qi, 17, [20, 50]) for _ in range(2))
+        batch = store.batch([0, 1], [4, 50])
+        if fault == "shared":
+            store.references[int(store.table[0, 0])] = 2
+        elif fault == "missing":
+            store.table[0, 0] = -1
+        elif fault == "foreign":
+            store.table[0, 0] = 1 << 30
+        elif fault == "count":
+            store.lengths[0] = 3
+        else:
+            batch.slots[0] = 2
+        rows, kv = make_kv(store, 54, torch.float16, 18)
+        append_plain(before, {w: x[4:] for w, x in kv.items()}, [1], [50])
+        assert qi.kv_append_ex(store.cache, store.pages, batch, 1, rows, rows[:, 256:], qi.DTYPE_F16, 512, 512) == 0
+        assert qi.kernel_status() >> 12 == 0x6C, fault
+        assert same_bytes(store, before), fault
+        assert qi.kernel_status() == 0
+
+
+# ---- pages -----------------------------------------------------------------------------------------------------------
+
+
+class Ledger:
+    """What the page calls do, on the CPU: tables, lengths, references, and what each page holds."""
+
+    def __init__(self, store):
+        self.store, self.page = store, store.page
+        self.table, self.lengths, self.references = store.table.tolist(), store.lengths.tolist(), store.references.tolist()
+        self.content = list(range(len(self.references)))
+
+    def free_pages(self):
+        return [p for p, n in enumerate(self.references) if n == 0]
+
+    def reserve(self, slots, counts):
+        need = [-(-(self.lengths[s] + c) // self.page) - -(-self.lengths[s] // self.page) for s, c in zip(slots, counts)]
+        free = self.free_pages()
+        if sum(need) > len(free):
+            return sum(need) - len(free)
+        for s, c, n in zip(slots, counts, need):
+            have = -(-self.lengths[s] // self.page)
+            for j in range(have, have + n):
+                self.table[s][j] = free.pop(0)
+                self.references[self.table[s][j]] = 1
+            self.lengths[s] += c
+        return 0
+
+    def fork(self, parents, children):
+        old, lengths, free = [row[:] for row in self.table], self.lengths[:], self.free_pages()
+        todo = [(p, c) for p, c in zip(parents, children) if p != c]
+        need = sum(lengths[p] % self.page > 0 for p, _ in todo)
+        if need > len(free):
+            return need - len(free)
+        content = self.content[:]
+        for p, c in todo:
+            for page in old[c]:
+                if page >= 0:
+                    self.references[page] -= 1
+            whole, row = lengths[p] // self.page, [-1] * len(old[c])
+            for j in range(whole):
+                row[j] = old[p][j]
+                self.references[row[j]] += 1
+            if lengths[p] % self.page:
+                row[whole] = free.pop(0)
+                self.references[row[whole]] = 1
+                self.content[row[whole]] = content[old[p][whole]]
+            self.table[c], self.lengths[c] = row, lengths[p]
+        return 0
+
+    def free(self, slots):
+        for s in slots:
+            for page in self.table[s]:
+                if page >= 0:
+                    self.references[page] -= 1
+            self.table[s], self.lengths[s] = [-1] * len(self.table[s]), 0
+
+    def compact(self):
+        used = sum(n > 0 for n in self.references)
+        sources = [p for p, n in enumerate(self.references) if n > 0 and p >= used]
+        targets = [p for p, n in enumerate(self.references) if n == 0 and p < used]
+        for a, b in zip(sources, targets):
+            self.references[b], self.references[a] = self.references[a], 0
+            self.content[b] = self.content[a]
+            self.table = [[b if page == a else page for page in row] for row in self.table]
+        return used
+
+    def check(self, start):
+        store = self.store
+        assert store.table.tolist() == self.table
+        assert store.lengths.tolist() == self.lengths
+        assert store.references.tolist() == self.references
+        content = torch.tensor(self.content, device="cuda")
+        for which in "kv":
+            assert torch.equal(store.codes[which], start[which + "c"][:, content])
+            assert torch.equal(store.scales[which].view(torch.int32), start[which + "s"][:, content].view(torch.int32))
+
+
+def pool_copy(store):
+    return {w + t: (store.codes if t == "c" else store.scales)[w].clone() for w in "kv" for t in "cs"}
+
+
+@pytest.mark.parametrize("seed,page,layers,kv_heads,head_dim", [(1, 16, 1, 1, 64), (2, 32, 3, 2, 128), (3, 64, 2, 5, 64), (4, 256, 2, 8, 128)])
+def test_pages_follow_the_ledger(qi, seed, page, layers, kv_heads, head_dim):
+    rng = random.Random(seed)
+    lengths = [rng.choice((0, 1, page - 1, page, page + 1, 3 * page, rng.randint(1, 5 * page))) for _ in range(23)]
+    store = Store(qi, seed, lengths, page=page, layers=layers, layer=0, kv_heads=kv_heads, head_dim=head_dim, spare=29, table_extra=3)
+    ledger, start = Ledger(store), pool_copy(store)
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda").fill_(0xA5)
+    told = ints([77])
+    for _ in range(12):
+        what = rng.choice(("reserve", "fork", "fork", "free", "compact", "permute"))
+        n = rng.randint(0, 9)
+        slots = rng.sample(range(23), n)
+        if what == "reserve":
+            width = store.table.shape[1] * page
+            slots = [s for s in slots if ledger.lengths[s] < width]
+            counts = [min(rng.choice((0, 1, 2, page, 2 * page + 1)), width - ledger.lengths[s]) for s in slots]
+            assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints(slots + [0]), ints(counts + [0]), len(slots), told, workspace) == 0
+            assert told.item() == ledger.reserve(slots, counts)
+        elif what in ("fork", "permute"):
+            parents = [rng.randrange(23) for _ in slots] if what == "fork" else rng.sample(slots, n)
+            assert qi.kv_pages_fork_ex(store.cache, store.pages, ints(parents + [0]), ints(slots + [0]), n, told, workspace) == 0
+            assert told.item() == ledger.fork(parents, slots)
+        elif what == "free":
+            assert qi.kv_pages_free_ex(store.cache, store.pages, ints(slots + [0]), n) == 0
+            ledger.free(slots)
+        else:
+            assert qi.kv_pages_compact_ex(store.cache, store.pages, told, workspace) == 0
+            assert told.item() == ledger.compact()
+        settled(qi)
+        ledger.check(start)
+
+
+def test_pages_that_do_not_suffice_change_nothing(qi):
+    store = Store(qi, 5, [40, 64, 33], page=32, spare=1, table_extra=4)
+    ledger, start = Ledger(store), pool_copy(store)
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda")
+    told = ints([0])
+    assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints([0, 1]), ints([60, 1]), 2, told, workspace) == 0
+    assert told.item() == 2
+    ledger.check(start)
+    assert qi.kv_pages_fork_ex(store.cache, store.pages, ints([0, 2]), ints([1, 0]), 2, told, workspace) == 0
+    assert told.item() == 1
+    ledger.check(start)
+    settled(qi)
+    # a list that is at fault: an unknown sequence, a negative count, more than a row of the table holds
+    for slots, counts in (([3], [1]), ([-1], [1]), ([0], [-1]), ([0], [32 * store.table.shape[1]]), ([0], [0x7fffffff])):
+        assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints(slots), ints(counts), 1, told, workspace) == 0
+        assert qi.kernel_status() >> 12 == 0x6C and told.item() == -1
+    assert qi.kv_pages_fork_ex(store.cache, store.pages, ints([0]), ints([9]), 1, told, workspace) == 0
+    assert qi.kernel_status() >> 12 == 0x6C and told.item() == -1
+    assert qi.kv_pages_free_ex(store.cache, store.pages, ints([9]), 1) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    ledger.check(start)
+
+
+def test_pages_of_a_large_pool(qi):
+    # more pages than one round of the planning CTA looks at, and a compaction that moves most of them
+    store = Store(qi, 6, [16 * 9] * 700, page=16, layers=1, layer=0, kv_heads=1, head_dim=64, spare=6000, table_extra=2)
+    ledger, start = Ledger(store), pool_copy(store)
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda")
+    told = ints([0])
+    gone = list(range(0, 700, 3))
+    assert qi.kv_pages_free_ex(store.cache, store.pages, ints(gone), len(gone)) == 0
+    ledger.free(gone)
+    assert qi.kv_pages_compact_ex(store.cache, store.pages, told, workspace) == 0
+    assert told.item() == ledger.compact()
+    more = list(range(700))
+    assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints(more), ints([17] * 700), 700, told, workspace) == 0
+    assert told.item() == ledger.reserve(more, [17] * 700) == 0
+    settled(qi)
+    ledger.check(start)
+
+
+def test_copying_pages(qi):
+    store = Store(qi, 7, [300], page=32, layers=3)
+    start = pool_copy(store)
+    assert qi.kv_pages_copy_ex(store.cache, ints([0, 3, 5]), ints([1, 4, 2]), 3) == 0
+    settled(qi)
+    for which in "kv":
+        for kind, now in (("c", store.codes[which]), ("s", store.scales[which])):
+            expected = start[which + kind].clone()
+            expected[:, [1, 4, 2]] = start[which + kind][:, [0, 3, 5]]
+            assert torch.equal(now.view(torch.uint8), expected.view(torch.uint8))
+    assert qi.kv_pages_copy_ex(store.cache, ints([0]), ints([99]), 1) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+
+
+# ---- norms -----------------------------------------------------------------------------------------------------------
+#
+# Tolerance. Everything is float32 but the stores: sums of w squares in a tree of at most 64 serial additions, 2^-18 of a positive sum, so a norm's
+# factor is within 2^-18; a handful of products and sums after it, 2^-22 each. With two norms in a row: 2^-16 of the largest term in magnitude.
+# float16 results add half a unit, 2^-11.
+
+
+def norm_exact(x, kind, epsilon, qi):
+    if kind == qi.NORM_LAYER:
+        x = x - x.mean(-1, keepdim=True)
+    return x / (x.square().mean(-1, keepdim=True) + epsilon).sqrt()
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,width", [(1, 8), (3, 64), (5, 1000), (2, 1024), (7, 2048), (300, 3080), (2, 4096), (9, 5120), (3, 8200), (2, 16384), (3000, 512)])
+def test_norms(qi, kind, rows, width):
+    kind = qi.NORM_LAYER if kind == "layer" else qi.NORM_RMS
+    g = torch.Generator(device="cuda").manual_seed(rows + width)
+    code = {torch.float16: qi.DTYPE_F16, torch.float32: qi.DTYPE_F32}
+    for case in range(6):
+        residual_type, branch_type, vector_type, y_type = (torch.float16 if case >> i & 1 else torch.float32 for i in range(4))
+        if case == 5:
+            residual_type, branch_type, vector_type, y_type = torch.float32, torch.float16, torch.float16, torch.float32
+        normal = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
+        residual, branch = (normal(rows, width) * 4 + 2).to(residual_type), (normal(rows, width) * 7 - 3).to(branch_type)
+        groups = 1 if case % 2 else 3
+        each = -(-rows // groups)
+        vectors = (normal(groups, 3 * width + 8) * 0.3).to(vector_type)
+        gate, scale, shift = (vectors[:, i * width:] if case != 2 else None for i in range(3))
+        branch_norm, weight = case in (0, 3, 5), normal(width) if case in (0, 1) else None
+        branch_weight = normal(width) if case in (0, 4) else None
+        out, y = torch.full_like(residual, float("nan")), torch.full((rows, width), float("nan"), dtype=y_type, device="cuda")
+        call = qi.GatedNorm(rows, width, kind=kind, epsilon=1e-5, residual=residual, residual_dtype=code[residual_type], branch=branch, branch_dtype=code[branch_type],
+                            branch_norm=branch_norm, branch_weight=branch_weight, residual_scale=0.7, gate=gate, scale=scale, shift=shift, vector_dtype=code[vector_type],
+                            ld_vector=3 * width + 8, rows_per_vector=each, weight=weight, residual_out=out, y=y, y_dtype=code[y_type])
+        assert qi.gated_norm_ex(call) == 0
+        settled(qi)
+        owner = torch.arange(rows, device="cuda") // each
+        b = branch.double()
+        if branch_norm:
+            b = norm_exact(b, kind, 1e-5, qi)
+        if branch_weight is not None:
+            b = b * branch_weight.double()
+        if gate is not None:
+            b = b * gate[owner, :width].double()
+        r = residual.double() + float(torch.tensor(0.7)) * b
+        n = norm_exact(r, kind, 1e-5, qi)
+        if weight is not None:
+            n = n * weight.double()
+        terms = n.abs()
+        if scale is not None:
+            n = n * (1 + scale[owner, :width].double())
+            terms = n.abs() + shift[owner, :width].double().abs()
+            n = n + shift[owner, :width].double()
+        for got, exact, size, dtype in ((out, r, residual.double().abs() + b.abs(), residual_type), (y, n, terms, y_type)):
+            bound = 2.0 ** -16 * size.amax(-1, keepdim=True) + (2.0 ** -11 * exact.abs() if dtype == torch.float16 else 0.0)
+            assert ((got.double() - exact).abs() <= bound).all(), (case, dtype)
+
+
+def test_norm_alone_in_place_and_on_another_stream(qi):
+    x, branch = torch.randn(50, 4096, device="cuda"), torch.randn(50, 4096, device="cuda")
+    expected, y = x + branch, torch.empty(50, 4096, dtype=torch.float16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    assert qi.gated_norm_ex(qi.GatedNorm(50, 4096, residual=x, branch=branch, residual_out=x, y=y, y_dtype=qi.DTYPE_F16), stream.cuda_stream) == 0
+    settled(qi)
+    assert torch.equal(x, expected)
+    alone = torch.empty_like(y)
+    assert qi.gated_norm_ex(qi.GatedNorm(50, 4096, residual=x, y=alone, y_dtype=qi.DTYPE_F16)) == 0
+    assert qi.gated_norm_ex(qi.GatedNorm(50, 4096, residual=x, branch=branch, residual_out=x)) == 0
+    settled(qi)
+    assert torch.equal(alone, y) and torch.equal(x, expected + branch)
+
+
+def test_norm_of_rows_without_spread(qi):
+    # a constant row has no deviation: epsilon keeps it finite; a large mean costs no digits of what is left
+    x = torch.full((3, 2048), 5.0, device="cuda")
+    x[1] = 0.0
+    x[2] = 1e4 + torch.randn(2048, device="cuda")
+    y = torch.empty_like(x)
+    assert qi.gated_norm_ex(qi.GatedNorm(3, 2048, kind=qi.NORM_LAYER, residual=x, y=y)) == 0
+    settled(qi)
+    assert (y[:2] == 0).all()
+    exact = norm_exact(x[2:].double(), qi.NORM_LAYER, 1e-6, qi)
+    assert (y[2:].double() - exact).abs().max() <= 2.0 ** -10  # a mean of 1e4 in 32 bits is known to 2^-11 of a deviation
