@@ -466,7 +466,7 @@ typedef struct {
 /* Writes new tokens into layer `layer`: row r of k and v [tokens, kv_heads, head_dim], ld_k and ld_v elements between rows
  * (multiples of 16 bytes), dtype QI_DTYPE_F32 or QI_DTYPE_F16. Their pages were reserved (qi_kv_pages_reserve_ex), so
  * lengths already count them, and no other sequence holds those pages. A block of 16 tokens and one head has
- *   scale = max |x| / 127 of its new tokens, or the scale of its earlier tokens if that is more,
+ *   scale = max |x| * (1 / 127) of its new tokens, or the scale of its earlier tokens if that is more,
  *   code  = rint(x / scale) + 128, earlier tokens again as rint((code - 128) * (old scale / scale)) + 128,
  * all in float32, ties to even. Writing the same tokens again changes nothing. x must be finite. */
 int qi_kv_append_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k,

@@ -7,6 +7,7 @@
 #include "kv_cache.cuh"
 #include "kv_decode.cuh"
 #include "kv_pages.cuh"
+#include "kv_prefill.cuh"
 
 namespace qi {
 namespace {
@@ -92,33 +93,47 @@ int launch_read(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_
 // ---- attention ----------------------------------------------------------------------------------------------------------
 
 struct AttentionPlan {
-    int tiles, rows, row_tiles, chunk, splits;
+    int tiles;  // of 8 query rows on mma.sync; 0: of 256 on tcgen05
+    int rows, row_tiles, chunk, splits;
     size_t partial_offset, bytes;
 };
+
+constexpr int DECODE_ROWS = 16;  // query rows to a sequence and head of the cache up to which a CTA of the streaming kernel holds all
 
 // How a call is cut: query rows into tiles, and the tokens of a tile into pieces where there are too few tiles for the GPU.
 bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int window, int sms, AttentionPlan &plan) {
     if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
     const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads);
-    plan.tiles = rows <= 8 ? 1 : 2;
-    plan.rows = 8 * plan.tiles;
+    plan.tiles = rows <= 8 ? 1 : rows <= DECODE_ROWS ? 2 : 0;
+    plan.rows = plan.tiles > 0 ? 8 * plan.tiles : kv::PREFILL_ROWS;
     const long long row_tiles = rows > 0 ? (rows + plan.rows - 1) / plan.rows : 1;
     if (row_tiles * cache->kv_heads > 65535) return false;
     plan.row_tiles = static_cast<int>(row_tiles);
     const long long units = row_tiles * cache->kv_heads * (batch->entries > 0 ? batch->entries : 1);
     long long span = max_length;  // of the tokens that a tile can see
     if (window > 0 && static_cast<long long>(window) + batch->most + kv::BLOCK < span) span = static_cast<long long>(window) + batch->most + kv::BLOCK;
-    const long long round = kv::DECODE_WARPS * kv::STEP, wanted = 12LL * sms;
-    long long chunk = (span * units + wanted - 1) / wanted;
+    // Pieces: streaming CTAs are small and many of them run at once; of the others one fills an SM, and pieces pay only while SMs are idle
+    const long long round = plan.tiles > 0 ? kv::DECODE_WARPS * kv::STEP : kv::TILE_TOKENS;
+    const long long pieces = plan.tiles > 0 ? (12LL * sms + units - 1) / units : sms / units > 1 ? sms / units : 1;
+    long long chunk = (span + pieces - 1) / pieces;
     chunk = (chunk + round - 1) / round * round;
     if (chunk < round) chunk = round;
-    long long splits = span > 0 ? (span + chunk - 1) / chunk : 1;
+    const long long splits = span > 0 ? (span + chunk - 1) / chunk : 1;
     plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(splits);
     plan.partial_offset = (static_cast<size_t>(units) * 4 + 255) / 256 * 256;
     // room for as many pieces as any window gives
-    const long long most = std::min((wanted + units - 1) / units, (max_length + round - 1) / round);
+    const long long most = std::min(pieces, (max_length + round - 1) / round);
     plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * plan.rows * (cache->head_dim + 2) * 4 : 0;
     return true;
+}
+
+template <int DIM>
+int launch_prefill(const dim3 grid, const kv::Cache &cache, const kv::Tables &tables, const kv::Batch &batch, const kv::Attention &a, void *stream) {
+    const int device = current_device();
+    if (device < 0) return static_cast<int>(cudaErrorNoDevice);
+    static std::atomic<bool> configured[MAX_DEVICES];
+    if (const cudaError_t error = configure_once(kv::prefill_kernel<DIM>, kv::Prefill<DIM>::SMEM_BYTES, configured[device])) return static_cast<int>(error);
+    return launch_grid(kv::prefill_kernel<DIM>, grid, kv::PREFILL_THREADS, kv::Prefill<DIM>::SMEM_BYTES, stream, cache, tables, batch, a);
 }
 
 kv::PageTables page_tables_of(const qi_kv_cache *cache, const qi_kv_pages *pages) {
@@ -203,9 +218,13 @@ int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const
     a.chunk = plan.chunk, a.splits = plan.splits, a.row_tiles = plan.row_tiles;
     a.arrivals = static_cast<int *>(workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.partial_offset);
+    const dim3 grid(plan.splits, cache->kv_heads * plan.row_tiles, batch->entries);
+    if (plan.tiles == 0)
+        return cache->head_dim == 128 ? launch_prefill<128>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream)
+                                      : launch_prefill<64>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream);
     auto kernel = cache->head_dim == 128 ? (plan.tiles == 1 ? kv::decode_kernel<128, 1> : kv::decode_kernel<128, 2>)
                                          : (plan.tiles == 1 ? kv::decode_kernel<64, 1> : kv::decode_kernel<64, 2>);
-    return launch_grid(kernel, dim3(plan.splits, cache->kv_heads * plan.row_tiles, batch->entries), kv::DECODE_THREADS, 0, stream, layer_of(cache, call->layer), tables_of(pages),
+    return launch_grid(kernel, grid, kv::DECODE_THREADS, 0, stream, layer_of(cache, call->layer), tables_of(pages),
                        batch_of(batch), a);
 }
 

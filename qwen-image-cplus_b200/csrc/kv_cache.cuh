@@ -62,7 +62,7 @@ __device__ __forceinline__ long long token_row(const Cache &cache, int page, int
 
 // ---- append ------------------------------------------------------------------------------------------------------
 //
-// scale = max |new value| / 127 over the new tokens of a block of 16 and all of a head's channels; where the block holds earlier
+// scale = max |new value| * (1 / 127) over the new tokens of a block of 16 and all of a head's channels; where the block holds earlier
 // tokens, at least the scale that they have, and if it is more, they are rounded again: rint(code * (old / new)). New codes are
 // rint(value / scale). A block's scale never falls while it holds earlier tokens, so writing the same tokens again changes nothing.
 //
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(Cache cache, 
     float *held = cache.scales[which] + row / BLOCK;
     peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));  // no negative ones: ordered as whole numbers
     const float old = early > 0 ? *held : 0.0f;
-    const float scale = fmaxf(old, __fdiv_rn(peak, 127.0f));
+    const float scale = fmaxf(old, __fmul_rn(peak, 1.0f / 127.0f));
     if (early > 0 && scale > old) {
         const float factor = __fdiv_rn(old, scale);
 #pragma unroll

@@ -247,7 +247,7 @@ def test_attention_in_a_graph_follows_lengths_on_the_device(qi, counts):
 
 # ---- append and read back ------------------------------------------------------------------------------------------
 #
-# Codes and scales are equal to the definition's in 32 bits, bit for bit: a division, a rounding and a product, each IEEE's.
+# Codes and scales are equal to the definition's in 32 bits, bit for bit: products, divisions and roundings, each IEEE's.
 
 
 def append_plain(store, kv, slots, counts):
@@ -263,7 +263,7 @@ def append_plain(store, kv, slots, counts):
             for which, x in kv.items():
                 new = x[begin + first - start:begin + end - start].float().cpu()
                 codes, scales = store.codes[which][store.layer, page].cpu(), store.scales[which][store.layer, page].cpu()
-                scale = new.abs().amax((0, 2)) / torch.tensor(127.0)
+                scale = new.abs().amax((0, 2)) * (1 / torch.tensor(127.0))
                 early = first - block * BLOCK
                 if early:
                     old = scales[:, within // BLOCK]
