@@ -8,11 +8,15 @@
 //                    scores were, the running maximum and sum in registers
 //   warps 8-11       widen codes: HBM -> registers -> float16 whole numbers in shared memory (exact), a tile ahead
 //   warp 12          issues the MMAs: S = Q K^T and O += P V, operands K and V from shared memory, P from TMEM
+//   warp 13          looks up pages and scales, up to four tiles ahead: page number, then scale, are two trips to memory in a row, and
+//                    where the widening warps made them they set the pace (4.3 us a tile and CTA instead of 2.5)
 // so that the two halves alternate: while one's weights are computed the tensor cores have the other's products. Values are stored as
 // they lie in the cache, a token a row, and enter their product "MN-major"; nothing is transposed.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (which then waits for the product before):
-// weights are at most 2^(8 + 7) in float16 and keep all their digits down to 2^-21 of that maximum; sums are float32.
+// m is not the maximum of what has been seen so far but an older one: weights are computed in one pass with the m that there is, and only
+// where those of 16 tokens add up to more than 2^15 (they are 2^7 where x = m, so that needs a growth by 2^4 to 2^8) is the tile's
+// maximum taken, O rescaled (which waits for the product before) and the pass repeated. So no weight is more than 2^15 in float16, and
+// all its digits are kept down to 2^-21 of the largest; sums are float32. Only the first tile pays for a pass over its maximum.
 //
 // TMEM: S and P of the halves at columns 0 and 128, O at 256 and 384.
 #pragma once
@@ -22,8 +26,8 @@ namespace qi {
 namespace kv {
 
 constexpr int PREFILL_THREADS = 512, TILE_ROWS = 128, TILE_TOKENS = 128, PREFILL_ROWS = 2 * TILE_ROWS;
-constexpr int WIDEN_WARP0 = 8, ISSUE_WARP = 12, TILE_BLOCKS = TILE_TOKENS / BLOCK, SCALE_SLOTS = 4;
-constexpr float PREFILL_SHIFT = 7.0f, GROWTH = 8.0f;
+constexpr int WIDEN_WARP0 = 8, ISSUE_WARP = 12, LOOK_UP_WARP = 13, TILE_BLOCKS = TILE_TOKENS / BLOCK, SLOTS = 4;
+constexpr float PREFILL_SHIFT = 7.0f, MOST_OF_BLOCK = 32768.0f;
 constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
 constexpr uint32_t TMEM_S = 0, TMEM_O = 256;
 
@@ -32,8 +36,8 @@ struct Prefill {
     static constexpr int HALVES = DIM / 64;                            // 128-byte rows of 64 channels
     static constexpr int OPERAND_BYTES = TILE_TOKENS * DIM * 2;        // of K, V, or half of Q
     static constexpr int Q_AT = 0, K_AT = 2 * OPERAND_BYTES, V_AT = 4 * OPERAND_BYTES, SCALES_AT = 6 * OPERAND_BYTES;
-    static constexpr int BARRIERS_AT = SCALES_AT + SCALE_SLOTS * 3 * TILE_BLOCKS * 4;
-    static constexpr int BARRIERS = 8 + SCALE_SLOTS + 6 + 1;
+    static constexpr int PLACES_AT = SCALES_AT + SLOTS * 3 * TILE_BLOCKS * 4, BARRIERS_AT = PLACES_AT + SLOTS * TILE_BLOCKS * 8;
+    static constexpr int BARRIERS = 8 + 2 * SLOTS + 6 + 1;
     static constexpr int SMEM_BYTES = BARRIERS_AT + BARRIERS * 8 + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
@@ -70,6 +74,11 @@ __device__ __forceinline__ void tmem_store_32x32(uint32_t address, const uint32_
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
         "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+__device__ __forceinline__ void tmem_store_32x16(uint32_t address, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(address), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -133,10 +142,11 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     using P = Prefill<DIM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float(*scales)[3][TILE_BLOCKS] = reinterpret_cast<float(*)[3][TILE_BLOCKS]>(smem + P::SCALES_AT);
+    float(*scales)[3][TILE_BLOCKS] = reinterpret_cast<float(*)[3][TILE_BLOCKS]>(smem + P::SCALES_AT);  // factor, offset, 1 / sv of each block
+    long long(*places)[TILE_BLOCKS] = reinterpret_cast<long long(*)[TILE_BLOCKS]>(smem + P::PLACES_AT);  // its token row; -1: none
     uint64_t *barriers = reinterpret_cast<uint64_t *>(smem + P::BARRIERS_AT);
-    uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *scale_full = barriers + 8;
-    uint64_t *s_full = barriers + 8 + SCALE_SLOTS, *p_full = s_full + 2, *o_done = s_full + 4, *q_full = s_full + 6;
+    uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *slot_full = barriers + 8, *slot_empty = slot_full + SLOTS;
+    uint64_t *s_full = slot_empty + SLOTS, *p_full = s_full + 2, *o_done = s_full + 4, *q_full = s_full + 6;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(barriers + P::BARRIERS);
     __shared__ int is_last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -150,7 +160,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             mbarrier_init(k_empty + i, 1), mbarrier_init(v_empty + i, 1);
             mbarrier_init(s_full + i, 1), mbarrier_init(p_full + i, 4), mbarrier_init(o_done + i, 1);
         }
-        for (int i = 0; i < SCALE_SLOTS; ++i) mbarrier_init(scale_full + i, 1);
+        for (int i = 0; i < SLOTS; ++i) mbarrier_init(slot_full + i, 1), mbarrier_init(slot_empty + i, 1);
         mbarrier_init(q_full, 8);
         fence_barrier_init();
     }
@@ -184,19 +194,12 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             setmaxnreg_dec<104>();
             constexpr int LANES = DIM / 16, TOKENS = 128 / LANES, LOADS = TILE_TOKENS / TOKENS;  // threads to a token, tokens and loads of a pass
             const int t = threadIdx.x - WIDEN_WARP0 * 32, row0 = t / LANES, chunk = t % LANES;
-            const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
             uint4 words[2][LOADS];  // of keys, of values
-            auto place_of = [&](int token) -> long long {  // token row of a block; -1: none
-                if (token >= end) return -1;
-                int page = __ldg(pages + (token >> cache.page_shift));
-                if (page < 0 || page >= cache.pages) complain(0xC041), page = 0;
-                return token_row(cache, page, head, token);
-            };
             auto fetch = [&](int which, int j) {
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const int token = begin + j * TILE_TOKENS + i * TOKENS + row0;
-                    const long long place = j < tiles ? place_of(token / BLOCK * BLOCK) : -1;
+                    const int token = i * TOKENS + row0;
+                    const long long place = j < tiles ? places[j % SLOTS][token / BLOCK] : -1;
                     words[which][i] = place < 0 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u)
                                                 : load_codes(cache.codes[which] + (place + token % BLOCK) * DIM + chunk * 16);
                 }
@@ -220,27 +223,16 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     }
                 }
             };
-            bool alive = true;
-            fetch(0, 0);
-            fetch(1, 0);
+            bool alive = tiles > 0 && mbarrier_wait_warp(slot_full, 0, &g_status, STATUS_WAIT_FULL | 0xC020, lane);
+            if (alive) fetch(0, 0), fetch(1, 0);
             for (int j = 0; j < tiles && alive; ++j) {
                 const int stage = j & 1, phase = j >> 1 & 1;
-                if (warp == WIDEN_WARP0) {
-                    if (lane < TILE_BLOCKS) {
-                        const long long place = place_of(begin + j * TILE_TOKENS + lane * BLOCK);
-                        const float k_scale = place < 0 ? 0.0f : __ldg(cache.scales[0] + place / BLOCK), v_scale = place < 0 ? 1.0f : fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE);
-                        scales[j % SCALE_SLOTS][0][lane] = fmaxf(k_scale * a.scale_log2, LEAST_FACTOR);
-                        scales[j % SCALE_SLOTS][1][lane] = log2f(v_scale);
-                        scales[j % SCALE_SLOTS][2][lane] = __frcp_rn(v_scale);
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbarrier_arrive(scale_full + j % SCALE_SLOTS);
-                }
                 if (!mbarrier_wait_warp(k_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC000 | stage, lane)) { alive = false; break; }
                 widen(0, smem_u32(smem + P::K_AT + stage * P::OPERAND_BYTES));
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbarrier_arrive(k_full + stage);
+                if (j + 1 < tiles && !mbarrier_wait_warp(slot_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
                 fetch(0, j + 1);
                 if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) { alive = false; break; }
                 widen(1, smem_u32(smem + P::V_AT + stage * P::OPERAND_BYTES));
@@ -277,7 +269,6 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     alive = mbarrier_wait_warp(v_full + stage, j >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC220 | stage, lane);
                     for (int i = 0; i < parts && alive; ++i) {
                         alive = mbarrier_wait_warp(p_full + i, j & 1, &g_status, STATUS_WAIT_READY | 0xC230 | i, lane);
-                        if (alive && i == 0 && j + 1 < tiles) alive = mbarrier_wait_warp(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next, lane);
                         if (!alive) break;
                         tcgen05_fence_after();
                         if (elected) {
@@ -286,14 +277,46 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                             for (int s = 0; s < TILE_TOKENS / 16; ++s)
                                 umma_f16_ts(tmem + TMEM_O + i * 128, tmem + TMEM_S + i * 128 + s * 8, umma_desc_mn_sw128(v + s * 2048, TILE_TOKENS * 128), IDESC_O, j > 0 || s > 0);
                             tcgen05_commit(o_done + i);
+                        }
+                        if (i == 0 && j + 1 < tiles) alive = mbarrier_wait_warp(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next, lane);
+                        if (!alive) break;
+                        tcgen05_fence_after();
+                        if (elected) {
                             if (j + 1 < tiles) scores(i, j + 1);
                             if (i == parts - 1) {
-                                tcgen05_commit(v_empty + stage);
+                                tcgen05_commit(v_empty + stage), tcgen05_commit(slot_empty + j % SLOTS);
                                 if (j + 1 < tiles) tcgen05_commit(k_empty + next);
                             }
                         }
                         __syncwarp();
                     }
+                }
+            } else if (warp == LOOK_UP_WARP) {
+                const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
+                auto page_at = [&](int j) {  // of this lane's block of tile j
+                    const int token = begin + j * TILE_TOKENS + lane * BLOCK;
+                    return lane < TILE_BLOCKS && token < end ? __ldg(pages + (token >> cache.page_shift)) : 0;
+                };
+                int page = page_at(0);
+                for (int j = 0; j < tiles; ++j) {
+                    const int next_page = page_at(j + 1), token = begin + j * TILE_TOKENS + lane * BLOCK;
+                    if (page < 0 || page >= cache.pages) complain(0xC041), page = 0;
+                    long long place = -1;
+                    float k_scale = 0.0f, v_scale = 1.0f;
+                    if (lane < TILE_BLOCKS && token < end) {
+                        place = token_row(cache, page, head, token);
+                        k_scale = __ldg(cache.scales[0] + place / BLOCK), v_scale = fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE);
+                    }
+                    if (j >= SLOTS && !mbarrier_wait_warp(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, &g_status, STATUS_WAIT_EMPTY | 0xC240, lane)) break;
+                    if (lane < TILE_BLOCKS) {
+                        places[j % SLOTS][lane] = place;
+                        scales[j % SLOTS][0][lane] = fmaxf(k_scale * a.scale_log2, LEAST_FACTOR);
+                        scales[j % SLOTS][1][lane] = log2f(v_scale);
+                        scales[j % SLOTS][2][lane] = __frcp_rn(v_scale);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbarrier_arrive(slot_full + j % SLOTS);
+                    page = next_page;
                 }
             }
         } else {
@@ -322,73 +345,100 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             bool alive = true;
             if (part < parts) {
                 for (int j = 0; j < tiles; ++j) {
-                    if (!mbarrier_wait_warp(scale_full + j % SCALE_SLOTS, j / SCALE_SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC300 | part, lane) ||
+                    if (!mbarrier_wait_warp(slot_full + j % SLOTS, j / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC300 | part, lane) ||
                         !mbarrier_wait_warp(s_full + part, j & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC300 | part, lane)) { alive = false; break; }
                     tcgen05_fence_after();
-                    uint32_t s[4][32];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_load_32x32(s_at + i * 32, s[i]);
-                    tmem_load_wait();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) arrived(s[i]);
-                    const float(&scale)[3][TILE_BLOCKS] = scales[j % SCALE_SLOTS];
+                    const float(&scale)[3][TILE_BLOCKS] = scales[j % SLOTS];
                     const int token = begin + j * TILE_TOKENS;
                     const int seen_low = row_low - token, seen_high = min(row_high, end) - token;
                     if (!__all_sync(0xffffffffu, seen_low <= 0 && seen_high >= TILE_TOKENS)) {
+                        // scores of hidden tokens become -infinity where they are: few tiles need it, and the others' code stays short
+#pragma unroll 1
+                        for (int k = 0; k < TILE_BLOCKS; ++k) {
+                            uint32_t hidden[BLOCK];
+                            tmem_load_32x16(s_at + k * BLOCK, hidden);
+                            tmem_load_wait();
+                            arrived(hidden);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int c = 0; c < 32; ++c)
-                                if (i * 32 + c < seen_low || i * 32 + c >= seen_high) s[i][c] = 0xff800000u;  // -infinity
-                    }
-                    float top = m;
-#pragma unroll
-                    for (int k = 0; k < TILE_BLOCKS; ++k) {
-                        float most = -INFINITY;
-#pragma unroll
-                        for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k / 2][k % 2 * BLOCK + c]));
-                        top = fmaxf(top, fmaf(most, scale[0][k], scale[1][k]));
-                    }
-                    const bool grown = top > m + GROWTH || (m == -INFINITY && top > m);
-                    if (__any_sync(0xffffffffu, grown)) {
-                        const float shrink = grown ? exp2_fast(m - top) : 1.0f;
-                        if (grown) m = top;
-                        if (j > 0) {
-                            if (!mbarrier_wait_warp(o_done + part, (j - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC310 | part, lane)) { alive = false; break; }
-                            tcgen05_fence_after();
-#pragma unroll
-                            for (int i = 0; i < DIM / 32; ++i) {
-                                uint32_t o[32];
-                                tmem_load_32x32(o_at + i * 32, o);
-                                tmem_load_wait();
-                                arrived(o);
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * shrink);
-                                tmem_store_32x32(o_at + i * 32, o);
-                            }
-                            l *= shrink;
+                            for (int c = 0; c < BLOCK; ++c)
+                                if (k * BLOCK + c < seen_low || k * BLOCK + c >= seen_high) hidden[c] = 0xff800000u;
+                            tmem_store_32x16(s_at + k * BLOCK, hidden);
                         }
+                        tmem_store_wait();
                     }
-                    const float base = m == -INFINITY ? 0.0f : m;
+                    // the 16 scores of a block; the next block's are on their way meanwhile
+                    uint32_t s[2][BLOCK];
+                    auto ask = [&](int k) { tmem_load_32x16(s_at + k * BLOCK, s[k & 1]); };
+                    auto take = [&](int k) {
+                        tmem_load_wait();
+                        arrived(s[k & 1]);
+                        if (k + 1 < TILE_BLOCKS) ask(k + 1);
+                    };
                     uint32_t p[2][32];
+                    float l_next;
+                    bool mine = m == -INFINITY, again = __any_sync(0xffffffffu, mine);  // a row that has seen nothing yet
+#pragma unroll 1
+                    while (true) {
+                        if (again) {  // the rows that want it take their maximum anew
+                            float top = m;
+                            ask(0);
 #pragma unroll
-                    for (int k = 0; k < TILE_BLOCKS; ++k) {
-                        const float factor = scale[0][k], offset = scale[1][k] - base + PREFILL_SHIFT;
-                        float sum = 0.0f;
+                            for (int k = 0; k < TILE_BLOCKS; ++k) {
+                                take(k);
+                                float most = -INFINITY;
 #pragma unroll
-                        for (int c = 0; c < BLOCK; c += 2) {
-                            float x[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float raw = __uint_as_float(s[k / 2][k % 2 * BLOCK + c + e]);
-                                x[e] = exp2_fast(fmaf(raw, factor, offset));
-                                sum += x[e];
+                                for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k & 1][c]));
+                                top = fmaxf(top, fmaf(most, scale[0][k], scale[1][k]));
                             }
-                            const __half2 pair = __floats2half2_rn(x[0], x[1]);
-                            p[k / 4][k % 4 * 8 + c / 2] = *reinterpret_cast<const uint32_t *>(&pair);
+                            const float shrink = mine && m != -INFINITY ? exp2_fast(m - top) : 1.0f;
+                            if (mine) m = top;
+                            if (j > 0) {
+                                alive = mbarrier_wait_warp(o_done + part, (j - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC310 | part, lane);
+                                if (!alive) break;
+                                tcgen05_fence_after();
+#pragma unroll 1
+                                for (int i = 0; i < DIM / 32; ++i) {
+                                    uint32_t o[32];
+                                    tmem_load_32x32(o_at + i * 32, o);
+                                    tmem_load_wait();
+                                    arrived(o);
+#pragma unroll
+                                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * shrink);
+                                    tmem_store_32x32(o_at + i * 32, o);
+                                }
+                                l *= shrink;
+                            }
                         }
-                        l = fmaf(sum, scale[2][k], l);
+                        const float base = m == -INFINITY ? 0.0f : m;
+                        float worst = 0.0f;
+                        l_next = l;
+                        ask(0);
+#pragma unroll
+                        for (int k = 0; k < TILE_BLOCKS; ++k) {
+                            take(k);
+                            const float factor = scale[0][k], offset = scale[1][k] - base + PREFILL_SHIFT;
+                            const uint64_t factors = pack_f32x2(factor, factor), offsets = pack_f32x2(offset, offset);
+                            uint64_t sums = pack_f32x2(0.0f, 0.0f);
+#pragma unroll
+                            for (int c = 0; c < BLOCK; c += 2) {
+                                float x, y;
+                                unpack_f32x2(fma_f32x2(pack_u32x2(s[k & 1][c], s[k & 1][c + 1]), factors, offsets), x, y);
+                                x = exp2_fast(x), y = exp2_fast(y);
+                                sums = add_f32x2(sums, pack_f32x2(x, y));
+                                const __half2 pair = __floats2half2_rn(x, y);
+                                p[k / 4][k % 4 * 8 + c / 2] = *reinterpret_cast<const uint32_t *>(&pair);
+                            }
+                            float even, odd;
+                            unpack_f32x2(sums, even, odd);
+                            worst = fmaxf(worst, even + odd);
+                            l_next = fmaf(even + odd, scale[2][k], l_next);
+                        }
+                        mine = !(worst <= MOST_OF_BLOCK);
+                        if (again || !__any_sync(0xffffffffu, mine)) break;
+                        again = true;
                     }
+                    if (!alive) break;
+                    l = l_next;
                     tmem_store_32x32(s_at, p[0]);
                     tmem_store_32x32(s_at + 32, p[1]);
                     tmem_store_wait();
