@@ -4,7 +4,7 @@
 //   y  = norm(r') * weight * (1 + scale) + shift           norm: x / rms(x), or (x - mean) / deviation
 //
 // Each row is read once and written once; the values stay in registers between the sums, which are float32 and taken about the
-// mean (two passes over registers, so that a large mean costs no digits). r' enters the second norm unrounded, also where it is
+// mean (passes over registers, so that a large mean costs no digits). r' enters the second norm unrounded, also where it is
 // stored as float16. Bound by memory: THREADS threads hold a row, 8 adjacent values a piece, so that every access is 16 bytes a thread or
 // more. CTAs walk over rows; the vectors (gate, scale, shift, weights) then come from L1, past which the rows are streamed.
 #pragma once
@@ -65,17 +65,17 @@ __device__ __forceinline__ void store8(void *base, bool f16, long long at, const
     }
 }
 
-// Sum over the CTA. Two rows of `sums` in turn: a thread that writes the next sum's has passed the barrier behind which all have
-// read the one before the last.
+// Two sums over the CTA. Two rows of `sums` in turn: a thread that writes the next sums' has passed the barrier behind which all have
+// read the ones before the last.
 template <int WARPS>
-__device__ __forceinline__ float block_sum(float value, float (&sums)[2][WARPS], int &turn) {
+__device__ __forceinline__ float2 block_sums(float2 value, float2 (&sums)[2][WARPS], int &turn) {
 #pragma unroll
-    for (int step = 16; step > 0; step /= 2) value += __shfl_xor_sync(0xffffffffu, value, step);
+    for (int step = 16; step > 0; step /= 2) value.x += __shfl_xor_sync(0xffffffffu, value.x, step), value.y += __shfl_xor_sync(0xffffffffu, value.y, step);
     if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = value;
     __syncthreads();
-    float total = 0.0f;
+    float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += sums[turn][w];
+    for (int w = 0; w < WARPS; ++w) total.x += sums[turn][w].x, total.y += sums[turn][w].y;
     turn ^= 1;
     return total;
 }
@@ -83,31 +83,38 @@ __device__ __forceinline__ float block_sum(float value, float (&sums)[2][WARPS],
 template <int THREADS, int PIECES>
 __global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
     constexpr int WARPS = THREADS / 32;
-    __shared__ float sums[2][WARPS];
+    __shared__ float2 sums[2][WARPS];
     grid_wait();
     int turn = 0;
     const float per_value = 1.0f / static_cast<float>(a.width);
-    // x becomes (x - mean if it is a layer norm) and its factor is returned
+    // x becomes (x - mean if it is a layer norm) and its factor is returned. The mean is taken twice, the second time of what the first
+    // left, together with the squares: a float32 sum of values around 10^4 knows their mean to 10^-3 only.
     auto normalise = [&](float (&x)[PIECES][8]) {
-        if (a.layer) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int p = 0; p < PIECES; ++p)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += x[p][j];
-            const float mean = block_sum<WARPS>(sum, sums, turn) * per_value;
+        auto shift_by = [&](float mean) {
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
                 if ((p * THREADS + static_cast<int>(threadIdx.x)) * 8 < a.width)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[p][j] -= mean;
+        };
+        float2 sum = make_float2(0.0f, 0.0f);
+        if (a.layer) {
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum.x += x[p][j];
+            shift_by(block_sums<WARPS>(sum, sums, turn).x * per_value);
+            sum.x = 0.0f;
         }
-        float squares = 0.0f;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) squares = fmaf(x[p][j], x[p][j], squares);
-        return rsqrtf(fmaf(block_sum<WARPS>(squares, sums, turn), per_value, a.epsilon));
+            for (int j = 0; j < 8; ++j) sum.x += x[p][j], sum.y = fmaf(x[p][j], x[p][j], sum.y);
+        sum = block_sums<WARPS>(sum, sums, turn);
+        if (!a.layer) return rsqrtf(fmaf(sum.y, per_value, a.epsilon));
+        const float rest = sum.x * per_value;
+        shift_by(rest);
+        return rsqrtf(fmaxf(fmaf(sum.y, per_value, -rest * rest), 0.0f) + a.epsilon);
     };
     for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long start = static_cast<long long>(row) * a.width, vector = static_cast<long long>(row / a.rows_per_vector) * a.ld_vector;

@@ -27,6 +27,7 @@ namespace kv {
 
 constexpr int PREFILL_THREADS = 512, TILE_ROWS = 128, TILE_TOKENS = 128, PREFILL_ROWS = 2 * TILE_ROWS;
 constexpr int WIDEN_WARP0 = 8, ISSUE_WARP = 12, LOOK_UP_WARP = 13, TILE_BLOCKS = TILE_TOKENS / BLOCK, SLOTS = 4;
+constexpr int HALF_TOKENS = TILE_TOKENS / 2, HALF_BLOCKS = TILE_BLOCKS / 2;
 constexpr float PREFILL_SHIFT = 7.0f, MOST_OF_BLOCK = 32768.0f;
 constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
 constexpr uint32_t TMEM_S = 0, TMEM_O = 256;
@@ -37,7 +38,7 @@ struct Prefill {
     static constexpr int OPERAND_BYTES = TILE_TOKENS * DIM * 2;        // of K, V, or half of Q
     static constexpr int Q_AT = 0, K_AT = 2 * OPERAND_BYTES, V_AT = 4 * OPERAND_BYTES, SCALES_AT = 6 * OPERAND_BYTES;
     static constexpr int PLACES_AT = SCALES_AT + SLOTS * 3 * TILE_BLOCKS * 4, BARRIERS_AT = PLACES_AT + SLOTS * TILE_BLOCKS * 8;
-    static constexpr int BARRIERS = 8 + 2 * SLOTS + 6 + 1;
+    static constexpr int BARRIERS = 8 + 2 * SLOTS + 10 + 1;
     static constexpr int SMEM_BYTES = BARRIERS_AT + BARRIERS * 8 + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     long long(*places)[TILE_BLOCKS] = reinterpret_cast<long long(*)[TILE_BLOCKS]>(smem + P::PLACES_AT);  // its token row; -1: none
     uint64_t *barriers = reinterpret_cast<uint64_t *>(smem + P::BARRIERS_AT);
     uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *slot_full = barriers + 8, *slot_empty = slot_full + SLOTS;
-    uint64_t *s_full = slot_empty + SLOTS, *p_full = s_full + 2, *o_done = s_full + 4, *q_full = s_full + 6;
+    uint64_t *s_full = slot_empty + SLOTS, *p_full = s_full + 2, *o_done = s_full + 6, *q_full = s_full + 10;  // of p and o [half of a tile][half of the rows]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(barriers + P::BARRIERS);
     __shared__ int is_last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -158,8 +159,9 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
         for (int i = 0; i < 2; ++i) {
             mbarrier_init(k_full + i, 4), mbarrier_init(v_full + i, 4);
             mbarrier_init(k_empty + i, 1), mbarrier_init(v_empty + i, 1);
-            mbarrier_init(s_full + i, 1), mbarrier_init(p_full + i, 4), mbarrier_init(o_done + i, 1);
+            mbarrier_init(s_full + i, 1);
         }
+        for (int i = 0; i < 4; ++i) mbarrier_init(p_full + i, 4), mbarrier_init(o_done + i, 1);
         for (int i = 0; i < SLOTS; ++i) mbarrier_init(slot_full + i, 1), mbarrier_init(slot_empty + i, 1);
         mbarrier_init(q_full, 8);
         fence_barrier_init();
@@ -268,17 +270,20 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     const int stage = j & 1, next = (j + 1) & 1;
                     alive = mbarrier_wait_warp(v_full + stage, j >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC220 | stage, lane);
                     for (int i = 0; i < parts && alive; ++i) {
-                        alive = mbarrier_wait_warp(p_full + i, j & 1, &g_status, STATUS_WAIT_READY | 0xC230 | i, lane);
-                        if (!alive) break;
-                        tcgen05_fence_after();
-                        if (elected) {
-                            const uint32_t v = v_at + stage * P::OPERAND_BYTES;
+                        for (int h = 0; h < 2; ++h) {
+                            alive = mbarrier_wait_warp(p_full + 2 * h + i, j & 1, &g_status, STATUS_WAIT_READY | 0xC230 | i, lane);
+                            if (!alive) break;
+                            tcgen05_fence_after();
+                            if (elected) {
+                                const uint32_t v = v_at + stage * P::OPERAND_BYTES + h * (HALF_TOKENS * 128), weights = tmem + TMEM_S + i * 128 + h * 32;
 #pragma unroll
-                            for (int s = 0; s < TILE_TOKENS / 16; ++s)
-                                umma_f16_ts(tmem + TMEM_O + i * 128, tmem + TMEM_S + i * 128 + s * 8, umma_desc_mn_sw128(v + s * 2048, TILE_TOKENS * 128), IDESC_O, j > 0 || s > 0);
-                            tcgen05_commit(o_done + i);
+                                for (int s = 0; s < HALF_TOKENS / 16; ++s)
+                                    umma_f16_ts(tmem + TMEM_O + i * 128, weights + s * 8, umma_desc_mn_sw128(v + s * 2048, TILE_TOKENS * 128), IDESC_O, j + h > 0 || s > 0);
+                                tcgen05_commit(o_done + 2 * h + i);
+                            }
+                            __syncwarp();
                         }
-                        if (i == 0 && j + 1 < tiles) alive = mbarrier_wait_warp(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next, lane);
+                        if (alive && i == 0 && j + 1 < tiles) alive = mbarrier_wait_warp(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next, lane);
                         if (!alive) break;
                         tcgen05_fence_after();
                         if (elected) {
@@ -348,7 +353,6 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     if (!mbarrier_wait_warp(slot_full + j % SLOTS, j / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC300 | part, lane) ||
                         !mbarrier_wait_warp(s_full + part, j & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC300 | part, lane)) { alive = false; break; }
                     tcgen05_fence_after();
-                    const float(&scale)[3][TILE_BLOCKS] = scales[j % SLOTS];
                     const int token = begin + j * TILE_TOKENS;
                     const int seen_low = row_low - token, seen_high = min(row_high, end) - token;
                     if (!__all_sync(0xffffffffu, seen_low <= 0 && seen_high >= TILE_TOKENS)) {
@@ -366,88 +370,93 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                         }
                         tmem_store_wait();
                     }
-                    // the 16 scores of a block; the next block's are on their way meanwhile
-                    uint32_t s[2][BLOCK];
-                    auto ask = [&](int k) { tmem_load_32x16(s_at + k * BLOCK, s[k & 1]); };
-                    auto take = [&](int k) {
-                        tmem_load_wait();
-                        arrived(s[k & 1]);
-                        if (k + 1 < TILE_BLOCKS) ask(k + 1);
-                    };
-                    uint32_t p[2][32];
-                    float l_next;
-                    bool mine = m == -INFINITY, again = __any_sync(0xffffffffu, mine);  // a row that has seen nothing yet
+                    // Half a tile at a time: the product of its first 64 tokens runs while the weights of the others are computed.
 #pragma unroll 1
-                    while (true) {
-                        if (again) {  // the rows that want it take their maximum anew
-                            float top = m;
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t half_at = s_at + h * HALF_TOKENS;
+                        const float(*factors)[TILE_BLOCKS] = &scales[j % SLOTS][0];
+                        const int first = h * HALF_BLOCKS;
+                        // the 16 scores of a block; the next block's are on their way meanwhile
+                        uint32_t s[2][BLOCK], p[32];
+                        auto ask = [&](int k) { tmem_load_32x16(half_at + k * BLOCK, s[k & 1]); };
+                        auto take = [&](int k) {
+                            tmem_load_wait();
+                            arrived(s[k & 1]);
+                            if (k + 1 < HALF_BLOCKS) ask(k + 1);
+                        };
+                        float l_next;
+                        bool again = __any_sync(0xffffffffu, m == -INFINITY);  // a row that has seen nothing yet
+#pragma unroll 1
+                        while (true) {
+                            if (again) {  // the maximum of every row, so that none can be over it below
+                                float top = m;
+                                ask(0);
+#pragma unroll
+                                for (int k = 0; k < HALF_BLOCKS; ++k) {
+                                    take(k);
+                                    float most = -INFINITY;
+#pragma unroll
+                                    for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k & 1][c]));
+                                    top = fmaxf(top, fmaf(most, factors[0][first + k], factors[1][first + k]));
+                                }
+                                const float shrink = m != -INFINITY ? exp2_fast(m - top) : 1.0f;
+                                m = top;
+                                if (j + h > 0) {
+                                    alive = mbarrier_wait_warp(o_done + 2 * (h ^ 1) + part, (h ? j : j - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC310 | part, lane);
+                                    if (!alive) break;
+                                    tcgen05_fence_after();
+#pragma unroll 1
+                                    for (int i = 0; i < DIM / 32; ++i) {
+                                        uint32_t o[32];
+                                        tmem_load_32x32(o_at + i * 32, o);
+                                        tmem_load_wait();
+                                        arrived(o);
+#pragma unroll
+                                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * shrink);
+                                        tmem_store_32x32(o_at + i * 32, o);
+                                    }
+                                    l *= shrink;
+                                }
+                            }
+                            const float base = (m == -INFINITY ? 0.0f : m) - PREFILL_SHIFT;
+                            float worst = 0.0f;
+                            l_next = l;
                             ask(0);
 #pragma unroll
-                            for (int k = 0; k < TILE_BLOCKS; ++k) {
+                            for (int k = 0; k < HALF_BLOCKS; ++k) {
                                 take(k);
-                                float most = -INFINITY;
+                                const float factor = factors[0][first + k], offset = factors[1][first + k] - base;
+                                const uint64_t factor2 = pack_f32x2(factor, factor), offset2 = pack_f32x2(offset, offset);
+                                uint64_t sums = pack_f32x2(0.0f, 0.0f);
 #pragma unroll
-                                for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k & 1][c]));
-                                top = fmaxf(top, fmaf(most, scale[0][k], scale[1][k]));
-                            }
-                            const float shrink = mine && m != -INFINITY ? exp2_fast(m - top) : 1.0f;
-                            if (mine) m = top;
-                            if (j > 0) {
-                                alive = mbarrier_wait_warp(o_done + part, (j - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC310 | part, lane);
-                                if (!alive) break;
-                                tcgen05_fence_after();
-#pragma unroll 1
-                                for (int i = 0; i < DIM / 32; ++i) {
-                                    uint32_t o[32];
-                                    tmem_load_32x32(o_at + i * 32, o);
-                                    tmem_load_wait();
-                                    arrived(o);
-#pragma unroll
-                                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * shrink);
-                                    tmem_store_32x32(o_at + i * 32, o);
+                                for (int c = 0; c < BLOCK; c += 2) {
+                                    float low, high;
+                                    unpack_f32x2(fma_f32x2(pack_u32x2(s[k & 1][c], s[k & 1][c + 1]), factor2, offset2), low, high);
+                                    low = exp2_fast(low), high = exp2_fast(high);
+                                    sums = add_f32x2(sums, pack_f32x2(low, high));
+                                    const __half2 pair = __floats2half2_rn(low, high);
+                                    p[(k * BLOCK + c) / 2] = *reinterpret_cast<const uint32_t *>(&pair);
                                 }
-                                l *= shrink;
+                                float even, odd;
+                                unpack_f32x2(sums, even, odd);
+                                worst = fmaxf(worst, even + odd);
+                                l_next = fmaf(even + odd, factors[2][first + k], l_next);
                             }
+                            if (again || __all_sync(0xffffffffu, worst <= MOST_OF_BLOCK)) break;
+                            again = true;
                         }
-                        const float base = m == -INFINITY ? 0.0f : m;
-                        float worst = 0.0f;
-                        l_next = l;
-                        ask(0);
-#pragma unroll
-                        for (int k = 0; k < TILE_BLOCKS; ++k) {
-                            take(k);
-                            const float factor = scale[0][k], offset = scale[1][k] - base + PREFILL_SHIFT;
-                            const uint64_t factors = pack_f32x2(factor, factor), offsets = pack_f32x2(offset, offset);
-                            uint64_t sums = pack_f32x2(0.0f, 0.0f);
-#pragma unroll
-                            for (int c = 0; c < BLOCK; c += 2) {
-                                float x, y;
-                                unpack_f32x2(fma_f32x2(pack_u32x2(s[k & 1][c], s[k & 1][c + 1]), factors, offsets), x, y);
-                                x = exp2_fast(x), y = exp2_fast(y);
-                                sums = add_f32x2(sums, pack_f32x2(x, y));
-                                const __half2 pair = __floats2half2_rn(x, y);
-                                p[k / 4][k % 4 * 8 + c / 2] = *reinterpret_cast<const uint32_t *>(&pair);
-                            }
-                            float even, odd;
-                            unpack_f32x2(sums, even, odd);
-                            worst = fmaxf(worst, even + odd);
-                            l_next = fmaf(even + odd, scale[2][k], l_next);
-                        }
-                        mine = !(worst <= MOST_OF_BLOCK);
-                        if (again || !__any_sync(0xffffffffu, mine)) break;
-                        again = true;
+                        if (!alive) break;
+                        l = l_next;
+                        tmem_store_32x32(s_at + h * 32, p);
+                        tmem_store_wait();
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbarrier_arrive(p_full + 2 * h + part);
                     }
                     if (!alive) break;
-                    l = l_next;
-                    tmem_store_32x32(s_at, p[0]);
-                    tmem_store_32x32(s_at + 32, p[1]);
-                    tmem_store_wait();
-                    tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbarrier_arrive(p_full + part);
                 }
                 if (alive && tiles > 0) {
-                    alive = mbarrier_wait_warp(o_done + part, (tiles - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC320 | part, lane);
+                    alive = mbarrier_wait_warp(o_done + 2 + part, (tiles - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC320 | part, lane);
                     tcgen05_fence_after();
                 }
                 const long long unit = (static_cast<long long>(b) * cache.heads + head) * a.row_tiles + tile;
