@@ -445,6 +445,11 @@ NORM_LAYER, NORM_RMS = 0, 1
 KV_BLOCK = 16  # tokens that share a scale
 
 
+def _address(pointer):
+    """What a void pointer argument takes, without an object around it: these calls are short."""
+    return pointer.data_ptr() if hasattr(pointer, "data_ptr") else pointer
+
+
 class KvCache:
     """The pool: codes uint8 [layers, pages, kv_heads, page_tokens, head_dim], scales float32 [layers, pages, kv_heads, page_tokens / 16]."""
 
@@ -456,6 +461,7 @@ class KvCache:
         if not all(t.is_contiguous() for t in (k_codes, v_codes, k_scales, v_scales)):
             raise ValueError("the codes and scales of a cache are contiguous")
         self.cache = qi_kv_cache(_p(k_codes), _p(v_codes), _p(k_scales), _p(v_scales), layers, pages, page_tokens, kv_heads, head_dim)
+        self.reference = ctypes.byref(self.cache)
 
 
 class KvPages:
@@ -467,6 +473,7 @@ class KvPages:
         if lengths.numel() != sequences or not all(t.is_contiguous() for t in (table, lengths, references)):
             raise ValueError("a table of pages, its lengths and its references are contiguous and belong together")
         self.pages = qi_kv_pages(_p(table), _p(lengths), _p(references), sequences, table_pages)
+        self.reference = ctypes.byref(self.pages)
 
 
 class KvBatch:
@@ -475,26 +482,27 @@ class KvBatch:
     def __init__(self, slots, offsets, tokens: int, most: int):
         self.slots, self.offsets = slots, offsets
         self.batch = qi_kv_batch(_p(slots), _p(offsets), offsets.numel() - 1, tokens, most)
+        self.reference = ctypes.byref(self.batch)
 
 
 def kv_append_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
     """Quantises the batch's keys and values into their pages."""
-    return lib().qi_kv_append_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), layer, _p(k), _p(v), dtype, ld_k, ld_v, _p(stream))
+    return lib().qi_kv_append_ex(cache.reference, pages.reference, batch.reference, layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
 
 
 def kv_read_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
     """The values that the cache holds for the batch's tokens."""
-    return lib().qi_kv_read_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), layer, _p(k), _p(v), dtype, ld_k, ld_v, _p(stream))
+    return lib().qi_kv_read_ex(cache.reference, pages.reference, batch.reference, layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
 
 
 def _bytes_of(workspace) -> int:
-    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+    return 0 if workspace is None else workspace.nbytes
 
 
 def kv_attention_workspace(cache: KvCache, batch: KvBatch, heads: int, max_length: int) -> int:
     """Bytes of workspace (to be zeroed once) that kv_attention_ex needs for batches within these bounds."""
     value = ctypes.c_size_t(0)
-    status = lib().qi_kv_attention_workspace(ctypes.byref(cache.cache), ctypes.byref(batch.batch), heads, max_length, ctypes.byref(value))
+    status = lib().qi_kv_attention_workspace(cache.reference, batch.reference, heads, max_length, ctypes.byref(value))
     if status != 0:
         raise ValueError(f"no attention of {heads} heads over such a cache (status {status})")
     return value.value
@@ -503,14 +511,14 @@ def kv_attention_workspace(cache: KvCache, batch: KvBatch, heads: int, max_lengt
 def kv_attention_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, q, ld_q: int, y, ld_y: int, heads: int, scale: float, max_length: int, *,
                     causal: bool = True, window: int = 0, lse=None, workspace=None, stream=None) -> int:
     """y = attention of float16 q over the batch's sequences; lse float32 [tokens, heads] or None."""
-    call = qi_kv_attention(layer, heads, _p(q), ld_q, _p(y), ld_y, _p(lse), scale, int(causal), window, max_length)
-    return lib().qi_kv_attention_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(batch.batch), ctypes.byref(call), _p(workspace), _bytes_of(workspace), _p(stream))
+    call = qi_kv_attention(layer, heads, _address(q), ld_q, _address(y), ld_y, _address(lse), scale, int(causal), window, max_length)
+    return lib().qi_kv_attention_ex(cache.reference, pages.reference, batch.reference, ctypes.byref(call), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_workspace(cache: KvCache, pages: KvPages) -> int:
     """Bytes of workspace of the calls below."""
     value = ctypes.c_size_t(0)
-    status = lib().qi_kv_pages_workspace(ctypes.byref(cache.cache), ctypes.byref(pages.pages), ctypes.byref(value))
+    status = lib().qi_kv_pages_workspace(cache.reference, pages.reference, ctypes.byref(value))
     if status != 0:
         raise ValueError(f"no such cache (status {status})")
     return value.value
@@ -518,27 +526,27 @@ def kv_pages_workspace(cache: KvCache, pages: KvPages) -> int:
 
 def kv_pages_reserve_ex(cache: KvCache, pages: KvPages, slots, counts, count: int, shortage, workspace, stream=None) -> int:
     """Pages for counts[i] more tokens of sequence slots[i]; `shortage` (device int32): 0, or how many pages are missing."""
-    return lib().qi_kv_pages_reserve_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(slots), _p(counts), count, _p(shortage), _p(workspace), _bytes_of(workspace), _p(stream))
+    return lib().qi_kv_pages_reserve_ex(cache.reference, pages.reference, _address(slots), _address(counts), count, _address(shortage), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_fork_ex(cache: KvCache, pages: KvPages, parents, children, count: int, shortage, workspace, stream=None) -> int:
     """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call."""
-    return lib().qi_kv_pages_fork_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(parents), _p(children), count, _p(shortage), _p(workspace), _bytes_of(workspace), _p(stream))
+    return lib().qi_kv_pages_fork_ex(cache.reference, pages.reference, _address(parents), _address(children), count, _address(shortage), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_free_ex(cache: KvCache, pages: KvPages, slots, count: int, stream=None) -> int:
     """The sequences end and give their pages back."""
-    return lib().qi_kv_pages_free_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(slots), count, _p(stream))
+    return lib().qi_kv_pages_free_ex(cache.reference, pages.reference, _address(slots), count, _address(stream))
 
 
 def kv_pages_compact_ex(cache: KvCache, pages: KvPages, used, workspace, stream=None) -> int:
     """Moves the pages in use together at the front; `used` (device int32) becomes their number."""
-    return lib().qi_kv_pages_compact_ex(ctypes.byref(cache.cache), ctypes.byref(pages.pages), _p(used), _p(workspace), _bytes_of(workspace), _p(stream))
+    return lib().qi_kv_pages_compact_ex(cache.reference, pages.reference, _address(used), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_copy_ex(cache: KvCache, sources, targets, count: int, stream=None) -> int:
     """Copies page sources[i] to page targets[i] in every layer."""
-    return lib().qi_kv_pages_copy_ex(ctypes.byref(cache.cache), _p(sources), _p(targets), count, _p(stream))
+    return lib().qi_kv_pages_copy_ex(cache.reference, _address(sources), _address(targets), count, _address(stream))
 
 
 class GatedNorm:
@@ -550,10 +558,11 @@ class GatedNorm:
         self.keep = (residual, branch, branch_weight, gate, scale, shift, weight, residual_out, y)
         self.call = qi_gated_norm(rows, width, kind, epsilon, _p(residual), residual_dtype, _p(branch), branch_dtype, int(branch_norm), _p(branch_weight), residual_scale, _p(gate),
                                   _p(scale), _p(shift), vector_dtype, ld_vector, rows_per_vector, _p(weight), _p(residual_out), _p(y), y_dtype)
+        self.reference = ctypes.byref(self.call)
 
 
 def gated_norm_ex(call: GatedNorm, stream=None) -> int:
-    return lib().qi_gated_norm_ex(ctypes.byref(call.call), _p(stream))
+    return lib().qi_gated_norm_ex(call.reference, _address(stream))
 
 
 # ---- the QIPACK v6 container (host side; int4_pack.cplus:36-95, 476-518, 733-850) ------------------------

@@ -114,7 +114,7 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     if (window > 0 && static_cast<long long>(window) + batch->most + kv::BLOCK < span) span = static_cast<long long>(window) + batch->most + kv::BLOCK;
     // Pieces: streaming CTAs are small and many of them run at once; of the others one fills an SM, and pieces pay only while SMs are idle
     const long long round = plan.tiles > 0 ? kv::DECODE_WARPS * kv::STEP : kv::TILE_TOKENS;
-    const long long pieces = plan.tiles > 0 ? (12LL * sms + units - 1) / units : sms / units > 1 ? sms / units : 1;
+    const long long pieces = plan.tiles > 0 ? (2LL * sms + units - 1) / units : sms / units > 1 ? sms / units : 1;
     long long chunk = (span + pieces - 1) / pieces;
     chunk = (chunk + round - 1) / round * round;
     if (chunk < round) chunk = round;
@@ -125,6 +125,15 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     const long long most = std::min(pieces, (max_length + round - 1) / round);
     plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * plan.rows * (cache->head_dim + 2) * 4 : 0;
     return true;
+}
+
+template <int DIM, int TILES>
+int launch_decode(const dim3 grid, const kv::Cache &cache, const kv::Tables &tables, const kv::Batch &batch, const kv::Attention &a, void *stream) {
+    const int device = current_device();
+    if (device < 0) return static_cast<int>(cudaErrorNoDevice);
+    static std::atomic<bool> configured[MAX_DEVICES];
+    if (const cudaError_t error = configure_once(kv::decode_kernel<DIM, TILES>, kv::Decode<DIM, TILES>::SMEM_BYTES, configured[device])) return static_cast<int>(error);
+    return launch_grid(kv::decode_kernel<DIM, TILES>, grid, kv::DECODE_THREADS, kv::Decode<DIM, TILES>::SMEM_BYTES, stream, cache, tables, batch, a);
 }
 
 template <int DIM>
@@ -222,10 +231,8 @@ int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const
     if (plan.tiles == 0)
         return cache->head_dim == 128 ? launch_prefill<128>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream)
                                       : launch_prefill<64>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream);
-    auto kernel = cache->head_dim == 128 ? (plan.tiles == 1 ? kv::decode_kernel<128, 1> : kv::decode_kernel<128, 2>)
-                                         : (plan.tiles == 1 ? kv::decode_kernel<64, 1> : kv::decode_kernel<64, 2>);
-    return launch_grid(kernel, grid, kv::DECODE_THREADS, 0, stream, layer_of(cache, call->layer), tables_of(pages),
-                       batch_of(batch), a);
+    auto launch = cache->head_dim == 128 ? (plan.tiles == 1 ? launch_decode<128, 1> : launch_decode<128, 2>) : (plan.tiles == 1 ? launch_decode<64, 1> : launch_decode<64, 2>);
+    return launch(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream);
 }
 
 int qi_kv_pages_workspace(const qi_kv_cache *cache, const qi_kv_pages *pages, size_t *bytes) {

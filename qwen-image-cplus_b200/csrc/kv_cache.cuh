@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(Cache cache, 
         }
     }
     const long long row = token_row(cache, page, head, block * BLOCK);
-    uint8_t *codes = cache.codes[which] + row * DIM + channel;
-    float *held = cache.scales[which] + row / BLOCK;
+    uint8_t *codes = (which == 0 ? cache.codes[0] : cache.codes[1]) + row * DIM + channel;
+    float *held = (which == 0 ? cache.scales[0] : cache.scales[1]) + row / BLOCK;
     peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));  // no negative ones: ordered as whole numbers
     const float old = early > 0 ? *held : 0.0f;
     const float scale = fmaxf(old, __fmul_rn(peak, 1.0f / 127.0f));
@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(Cache cache, Tables 
             continue;
         }
         const long long row = token_row(cache, page, head, token);
-        words[i] = *reinterpret_cast<const uint32_t *>(cache.codes[which] + row * DIM + rest % QUADS * 4);
-        scales[i] = cache.scales[which][row / BLOCK];
+        words[i] = *reinterpret_cast<const uint32_t *>((which == 0 ? cache.codes[0] : cache.codes[1]) + row * DIM + rest % QUADS * 4);
+        scales[i] = (which == 0 ? cache.scales[0] : cache.scales[1])[row / BLOCK];
     }
 #pragma unroll
     for (int i = 0; i < READ_ROWS; ++i) {

@@ -9,13 +9,15 @@
 // The products run transposed on m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an instruction are tokens and channels
 // of the cache, of which there are always enough, and the 8 columns are queries, of which there may be one. Which channel or
 // token stands at which place of a sum is free as long as both operands agree, and is chosen so that every load is 16 adjacent
-// codes of a token: codes go from HBM to registers and from there, widened, into the tensor cores, never through shared memory.
+// codes of a token: codes go as they are through shared memory and are widened in registers.
 //
 // Scales cost nothing per element. With base-2 logarithms, x_j = (scale * log2 e * sk) * raw_j + log2 sv, m = max x_j, p_j = 2^(x_j - m):
 //   O = sum p_j d_j (d_j whole numbers),  l = sum p_j / sv,  y = O / l
 // so sk and log2 sv enter one fused multiply-add, and 1 / sv once for the sum of a block. p_j is rounded to float16 for the tensor
-// cores, in a range shifted up by 2^12 so that it keeps all its digits down to 2^-26 of the largest; queries are float16 as they
-// come, codes are exact, all sums are float32. A block of zeros has sv = 0: log2 is taken of max(sv, 2^-60), which changes
+// cores; queries are float16 as they come, codes are exact, all sums are float32. m is not the maximum of what has been seen so far but an
+// older one: weights are computed with the m that there is, as 2^(x - m + 7), and only where one of them could be more than 2^15 is
+// the maximum taken anew and O rescaled. So float16 weights neither run over nor lose digits above 2^-21 of the largest, and what every
+// step would spend on a maximum over the warp (shuffles, one after the other) is spent in the first. A block of zeros has sv = 0: log2 is taken of max(sv, 2^-60), which changes
 // nothing that float16 results could hold.
 #pragma once
 #include "kv_cache.cuh"
@@ -23,7 +25,8 @@
 namespace qi {
 namespace kv {
 
-constexpr float P_SHIFT = 12.0f, LEAST_SCALE = 8.6736174e-19f;  // 2^-60
+constexpr float P_SHIFT = 7.0f, MOST_SUM = 32768.0f, LEAST_SCALE = 8.6736174e-19f;  // 2^-60
+constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
 constexpr int DECODE_WARPS = 4, DECODE_THREADS = DECODE_WARPS * 32, STEP = 32;
 
 struct Attention {
@@ -42,6 +45,17 @@ struct Attention {
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -69,12 +83,6 @@ __device__ __forceinline__ uint4 load_codes(const uint8_t *at) {  // read once b
     asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(at));
     return w;
 }
-__device__ __forceinline__ uint2 load_codes8(const uint8_t *at) {
-    uint2 w;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(at));
-    return w;
-}
-
 // The keys that row `row` of an entry (row = token * group + head of the group) sees: [low, high).
 __device__ __forceinline__ void visible(const Attention &a, const Entry &entry, int row, int &low, int &high) {
     const int position = entry.length - entry.count + row / a.group;
@@ -83,12 +91,31 @@ __device__ __forceinline__ void visible(const Attention &a, const Entry &entry, 
 }
 
 template <int DIM, int TILES>
-__global__ void __launch_bounds__(DECODE_THREADS, TILES == 1 ? 3 : 2) decode_kernel(Cache cache, Tables tables, Batch batch, Attention a) {
+struct Decode {
+    static constexpr int STAGES = DIM == 128 ? 3 : 5, STAGE_BYTES = 2 * STEP * DIM + 32;  // codes of keys, of values, scales
+    struct Join {
+        float o[DECODE_WARPS][8 * TILES][DIM + 4], m[DECODE_WARPS][8 * TILES], l[DECODE_WARPS][8 * TILES];
+    };
+    static constexpr int SMEM_BYTES = DECODE_WARPS * STAGES * STAGE_BYTES;
+    static_assert(sizeof(Join) <= SMEM_BYTES, "warps are joined where their rings were");
+};
+
+// Where piece `piece` (16 bytes) of a token's codes lies in its row: keys are read by lanes of two tokens in turn with four pieces each, values
+// by lanes of four tokens, two apart, with two pieces each.
+template <int DIM>
+__device__ __forceinline__ int key_place(int token, int piece) { return DIM == 128 ? piece ^ (token & 1) << 2 : piece; }
+template <int DIM>
+__device__ __forceinline__ int value_place(int token, int piece) { return DIM == 128 ? piece ^ (token >> 1 & 3) << 1 : piece ^ (token >> 1 & 3); }
+
+template <int DIM, int TILES>
+__global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, Tables tables, Batch batch, Attention a) {
     constexpr int ROWS = 8 * TILES, K_WORDS = DIM / 16;            // K_WORDS: 32-bit words of a token's codes that a lane holds (keys)
     constexpr int V_WORDS = DIM / 32, BLOCKS = STEP / BLOCK;       // and of values, of each of four tokens
-    constexpr int PITCH = DIM + 4;
-    __shared__ float join_o[DECODE_WARPS][ROWS][PITCH];
-    __shared__ float join_m[DECODE_WARPS][ROWS], join_l[DECODE_WARPS][ROWS];
+    constexpr int STAGES = Decode<DIM, TILES>::STAGES, STAGE_BYTES = Decode<DIM, TILES>::STAGE_BYTES;
+    extern __shared__ uint8_t smem[];
+    using Join = typename Decode<DIM, TILES>::Join;
+    auto &join_o = reinterpret_cast<Join *>(smem)->o;
+    auto &join_m = reinterpret_cast<Join *>(smem)->m, &join_l = reinterpret_cast<Join *>(smem)->l;
     __shared__ int is_last;
     grid_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row8 = lane >> 2, quad = lane & 3;
@@ -141,78 +168,71 @@ __global__ void __launch_bounds__(DECODE_THREADS, TILES == 1 ? 3 : 2) decode_ker
     }
 
     const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
-    long long place[BLOCKS];   // token row of each block of the step whose codes are fetched next; -1: none
+    // Each warp has a ring of STAGES steps of its own in shared memory, filled by 16-byte asynchronous copies, 16 KB of them under way at
+    // any time. Pieces of a row are stored where eight lanes that read together meet no bank twice (DIM 64, values: two of them do).
+    uint8_t *ring = smem + warp * (STAGES * STAGE_BYTES);
+    auto place_of = [&](int token) -> long long {  // token row of a block; -1: none
+        if (token >= end) return -1;
+        int page = __ldg(pages + (token >> cache.page_shift));
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.pages)) complain(0xC031), page = 0;
+        return token_row(cache, page, head, token);
+    };
+    const bool one_page = cache.page_shift >= 5 && begin % STEP == 0;  // a step's blocks follow each other in memory
+    long long place[BLOCKS];                                           // of the step that is fetched next
     auto look_up = [&](int token) {
+        place[0] = place_of(token);
+        if (one_page) place[1] = token + BLOCK < end ? place[0] + BLOCK : -1;
+        else place[1] = place_of(token + BLOCK);
+    };
+    static_assert(BLOCKS == 2, "look_up");
+    auto fetch = [&](int step) {  // the step's codes and scales, from `place`
+        uint8_t *stage = ring + step % STAGES * STAGE_BYTES;
 #pragma unroll
         for (int k = 0; k < BLOCKS; ++k) {
-            place[k] = -1;
-            if (token + k * BLOCK < end) {
-                int page = __ldg(pages + (token + k * BLOCK >> cache.page_shift));
-                if (page < 0 || page >= cache.pages) complain(0xC031), page = 0;
-                place[k] = token_row(cache, page, head, token + k * BLOCK);
+            if (place[k] >= 0) {
+                constexpr int PIECES = DIM / 16, TOKENS = 32 / PIECES;  // 16-byte pieces of a token, tokens a pass
+                const int piece = lane % PIECES, row = lane / PIECES;
+#pragma unroll
+                for (int i = 0; i < BLOCK / TOKENS; ++i) {
+                    const int t = i * TOKENS + row;
+                    cp_async_16(stage + (k * BLOCK + t) * DIM + key_place<DIM>(t, piece) * 16, cache.codes[0] + (place[k] + t) * DIM + piece * 16);
+                    cp_async_16(stage + (STEP + k * BLOCK + t) * DIM + value_place<DIM>(t, piece) * 16, cache.codes[1] + (place[k] + t) * DIM + piece * 16);
+                }
+                if (lane < 2) cp_async_4(stage + 2 * STEP * DIM + (2 * k + lane) * 4, (lane == 0 ? cache.scales[0] : cache.scales[1]) + place[k] / BLOCK);
             }
         }
-    };
-    uint32_t key[BLOCKS][2][K_WORDS], value[BLOCKS][4][V_WORDS];
-    float k_scale[BLOCKS], v_scale[BLOCKS];
-    long long value_place[BLOCKS];
-    auto fetch_keys = [&]() {
-#pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            value_place[k] = place[k];
-            k_scale[k] = 0.0f, v_scale[k] = 1.0f;
-            if (place[k] < 0) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < K_WORDS; ++j) key[k][i][j] = 0x80808080u;
-                continue;
-            }
-            k_scale[k] = __ldg(cache.scales[0] + place[k] / BLOCK), v_scale[k] = __ldg(cache.scales[1] + place[k] / BLOCK);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < DIM / 64; ++j) {
-                    const uint4 w = load_codes(cache.codes[0] + (place[k] + row8 + 8 * i) * DIM + (quad + 4 * j) * 16);
-                    key[k][i][4 * j] = w.x, key[k][i][4 * j + 1] = w.y, key[k][i][4 * j + 2] = w.z, key[k][i][4 * j + 3] = w.w;
-                }
-        }
-    };
-    auto fetch_values = [&]() {
-#pragma unroll
-        for (int k = 0; k < BLOCKS; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (value_place[k] < 0) {
-#pragma unroll
-                    for (int j = 0; j < V_WORDS; ++j) value[k][i][j] = 0x80808080u;
-                    continue;
-                }
-                const uint8_t *at = cache.codes[1] + (value_place[k] + quad * 2 + (i & 1) + 8 * (i >> 1)) * DIM + row8 * (DIM / 8);
-                if constexpr (DIM == 128) {
-                    const uint4 w = load_codes(at);
-                    value[k][i][0] = w.x, value[k][i][1] = w.y, value[k][i][2] = w.z, value[k][i][3] = w.w;
-                } else {
-                    const uint2 w = load_codes8(at);
-                    value[k][i][0] = w.x, value[k][i][1] = w.y;
-                }
-            }
+        cp_async_commit();
     };
 
     int token = begin + warp * STEP;
     look_up(token);
-    fetch_keys();
-    fetch_values();
-    look_up(token + DECODE_THREADS);
-    for (; token < end; token += DECODE_THREADS) {
+    for (int step = 0; step < STAGES - 1; ++step) {
+        fetch(step);
+        look_up(token + (step + 1) * DECODE_THREADS);
+    }
+    int step = 0;
+    for (; token < end; token += DECODE_THREADS, ++step) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();  // the step is there for every lane, and the one before it is done with
+        fetch(step + STAGES - 1);
+        look_up(token + STAGES * DECODE_THREADS);
+        const uint8_t *stage = ring + step % STAGES * STAGE_BYTES;
         float s[TILES][BLOCKS][4];
 #pragma unroll
         for (int k = 0; k < BLOCKS; ++k) {
 #pragma unroll
             for (int n = 0; n < TILES; ++n) s[n][k][0] = s[n][k][1] = s[n][k][2] = s[n][k][3] = 0.0f;
+            uint32_t key[2][K_WORDS];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < DIM / 64; ++j) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + (k * BLOCK + row8 + 8 * i) * DIM + key_place<DIM>(row8, quad + 4 * j) * 16);
+                    key[i][4 * j] = w.x, key[i][4 * j + 1] = w.y, key[i][4 * j + 2] = w.z, key[i][4 * j + 3] = w.w;
+                }
 #pragma unroll
             for (int j = 0; j < K_WORDS; ++j) {
-                const uint32_t a0 = widen2<0x4140>(key[k][0][j]), a1 = widen2<0x4140>(key[k][1][j]), a2 = widen2<0x4342>(key[k][0][j]), a3 = widen2<0x4342>(key[k][1][j]);
+                const uint32_t a0 = widen2<0x4140>(key[0][j]), a1 = widen2<0x4140>(key[1][j]), a2 = widen2<0x4342>(key[0][j]), a3 = widen2<0x4342>(key[1][j]);
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) mma_16x8x16(s[n][k], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
             }
@@ -220,58 +240,97 @@ __global__ void __launch_bounds__(DECODE_THREADS, TILES == 1 ? 3 : 2) decode_ker
         float factor[BLOCKS], offset[BLOCKS], inverse[BLOCKS];
 #pragma unroll
         for (int k = 0; k < BLOCKS; ++k) {
-            const float scale = fmaxf(v_scale[k], LEAST_SCALE);
-            factor[k] = k_scale[k] * a.scale_log2, offset[k] = log2f(scale), inverse[k] = __frcp_rn(scale);
+            const float2 scales = *reinterpret_cast<const float2 *>(stage + 2 * STEP * DIM + 8 * k);
+            const bool there = token + k * BLOCK < end;
+            const float scale = there ? fmaxf(scales.y, LEAST_SCALE) : 1.0f;
+            factor[k] = there ? scales.x * a.scale_log2 : 0.0f, offset[k] = log2_fast(scale), inverse[k] = reciprocal_fast(scale);
         }
-        fetch_keys();
-        const bool whole = token >= all_low && token + STEP <= min(all_high, end);
+        if (!(token >= all_low && token + STEP <= min(all_high, end))) {
+            // what is hidden: its score becomes -infinity, and the block's factor, if it is 0, something that leaves it that
+#pragma unroll
+            for (int k = 0; k < BLOCKS; ++k) {
+                factor[k] = fmaxf(factor[k], LEAST_FACTOR);
+#pragma unroll
+                for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = token + k * BLOCK + row8 + i / 2 * 8;
+                        if (at < row_low[n][i & 1] || at >= min(row_high[n][i & 1], end)) s[n][k][i] = -INFINITY;
+                    }
+            }
+        }
+        float weight[TILES][BLOCKS][4], l_next[TILES][2];
+        bool nothing = false;  // a row that has seen nothing yet
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) nothing |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+        bool again = __any_sync(0xffffffffu, nothing);
+        while (true) {
+            if (again) {
+#pragma unroll
+                for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = m[n][i];
+#pragma unroll
+                        for (int k = 0; k < BLOCKS; ++k) top = fmaxf(top, fmaf(fmaxf(s[n][k][i], s[n][k][2 + i]), factor[k], offset[k]));
+#pragma unroll
+                        for (int step = 4; step < 32; step *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+                        const float shrink = m[n][i] == -INFINITY ? 1.0f : exp2_fast(m[n][i] - top);
+                        m[n][i] = top, l[n][i] *= shrink;
+#pragma unroll
+                        for (int t = 0; t < DIM / 16; ++t) o[n][t][i] *= shrink, o[n][t][2 + i] *= shrink;
+                    }
+            }
+            float worst = 0.0f;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float base = (m[n][i] == -INFINITY ? 0.0f : m[n][i]) - P_SHIFT;
+                    l_next[n][i] = l[n][i];
+#pragma unroll
+                    for (int k = 0; k < BLOCKS; ++k) {
+                        weight[n][k][i] = exp2_fast(fmaf(s[n][k][i], factor[k], offset[k] - base)), weight[n][k][2 + i] = exp2_fast(fmaf(s[n][k][2 + i], factor[k], offset[k] - base));
+                        const float sum = weight[n][k][i] + weight[n][k][2 + i];
+                        worst = fmaxf(worst, sum);
+                        l_next[n][i] = fmaf(sum, inverse[k], l_next[n][i]);
+                    }
+                }
+            if (again || __all_sync(0xffffffffu, worst <= MOST_SUM)) break;
+            again = true;
+        }
         uint32_t p[TILES][BLOCKS][2];
 #pragma unroll
-        for (int n = 0; n < TILES; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float top = m[n][i];
-#pragma unroll
-                for (int k = 0; k < BLOCKS; ++k)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float &x = s[n][k][2 * r + i];
-                        x = fmaf(x, factor[k], offset[k]);
-                        const int at = token + k * BLOCK + row8 + 8 * r;
-                        if (!whole && (at < row_low[n][i] || at >= min(row_high[n][i], end))) x = -INFINITY;
-                        top = fmaxf(top, x);
-                    }
-#pragma unroll
-                for (int step = 4; step < 32; step *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-                const float base = top == -INFINITY ? 0.0f : top;
-                const float shrink = exp2_fast(m[n][i] - base);
-                m[n][i] = top;
-                l[n][i] *= shrink;
-#pragma unroll
-                for (int t = 0; t < DIM / 16; ++t) o[n][t][i] *= shrink, o[n][t][2 + i] *= shrink;
-#pragma unroll
-                for (int k = 0; k < BLOCKS; ++k) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) s[n][k][2 * r + i] = exp2_fast(s[n][k][2 * r + i] - (base - P_SHIFT));
-                    l[n][i] = fmaf(s[n][k][i] + s[n][k][2 + i], inverse[k], l[n][i]);
-                }
-            }
-#pragma unroll
-        for (int n = 0; n < TILES; ++n)
+        for (int n = 0; n < TILES; ++n) {
+            l[n][0] = l_next[n][0], l[n][1] = l_next[n][1];
 #pragma unroll
             for (int k = 0; k < BLOCKS; ++k)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const __half2 pair = __floats2half2_rn(s[n][k][2 * r], s[n][k][2 * r + 1]);
+                    const __half2 pair = __floats2half2_rn(weight[n][k][2 * r], weight[n][k][2 * r + 1]);
                     p[n][k][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&pair));
                 }
+        }
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k)
+        for (int k = 0; k < BLOCKS; ++k) {
+            uint32_t value[4][V_WORDS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = quad * 2 + (i & 1) + 8 * (i >> 1);
+                const uint8_t *at = stage + (STEP + k * BLOCK + t) * DIM + value_place<DIM>(t, row8 * DIM / 128) * 16;
+                if constexpr (DIM == 128) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(at);
+                    value[i][0] = w.x, value[i][1] = w.y, value[i][2] = w.z, value[i][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(at + row8 % 2 * 8);
+                    value[i][0] = w.x, value[i][1] = w.y;
+                }
+            }
 #pragma unroll
             for (int w = 0; w < V_WORDS; ++w) {
                 // [channel 4w of two tokens, channel 4w + 1 of both], and 4w + 2, 4w + 3; tokens 8 further on likewise
-                const uint32_t low0 = __byte_perm(value[k][0][w], value[k][1][w], 0x5140), high0 = __byte_perm(value[k][0][w], value[k][1][w], 0x7362);
-                const uint32_t low8 = __byte_perm(value[k][2][w], value[k][3][w], 0x5140), high8 = __byte_perm(value[k][2][w], value[k][3][w], 0x7362);
+                const uint32_t low0 = __byte_perm(value[0][w], value[1][w], 0x5140), high0 = __byte_perm(value[0][w], value[1][w], 0x7362);
+                const uint32_t low8 = __byte_perm(value[2][w], value[3][w], 0x5140), high8 = __byte_perm(value[2][w], value[3][w], 0x7362);
                 const uint32_t a0 = widen2<0x4140>(low0), a1 = widen2<0x4342>(low0), a2 = widen2<0x4140>(low8), a3 = widen2<0x4342>(low8);
                 const uint32_t c0 = widen2<0x4140>(high0), c1 = widen2<0x4342>(high0), c2 = widen2<0x4140>(high8), c3 = widen2<0x4342>(high8);
 #pragma unroll
@@ -280,9 +339,10 @@ __global__ void __launch_bounds__(DECODE_THREADS, TILES == 1 ? 3 : 2) decode_ker
                     mma_16x8x16(o[n][2 * w + 1], c0, c1, c2, c3, p[n][k][0], p[n][k][1]);
                 }
             }
-        fetch_values();
-        look_up(token + 2 * DECODE_THREADS);
+        }
     }
+    cp_async_wait<0>();
+    __syncthreads();  // the rings become the place where warps are joined
 
     // warps, then pieces
 #pragma unroll
@@ -336,49 +396,53 @@ __global__ void __launch_bounds__(DECODE_THREADS, TILES == 1 ? 3 : 2) decode_ker
     __syncthreads();
     if (!is_last) return;
     __threadfence();
-    // Warps share the pieces, lanes the channels: many loads on their way at once, where a thread that walked through all pieces of
-    // its channels took 70 us for 200 of them.
-    constexpr int PIECE = ROWS * (DIM + 2), EACH = DIM / 32;
-    float top[ROWS], total[ROWS], sum[ROWS][EACH];
+    // Warps share the pieces, lanes the channels, four rows at a time (the last again where there are fewer: no branch stands between
+    // one load and the next, of which there have to be many under way; with a walk over rows one by one this took 17 us for 37 pieces).
+    constexpr int PIECE = ROWS * (DIM + 2), EACH = DIM / 32, AT_ONCE = 4;
+    for (int first = 0; first < owned; first += AT_ONCE) {
+        float top[AT_ONCE], total[AT_ONCE], sum[AT_ONCE][EACH];
+        int rows_of[AT_ONCE];
 #pragma unroll
-    for (int row = 0; row < ROWS; ++row) {
-        top[row] = -INFINITY, total[row] = 0.0f;
+        for (int r = 0; r < AT_ONCE; ++r) {
+            rows_of[r] = min(first + r, owned - 1);
+            top[r] = -INFINITY, total[r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < EACH; ++c) sum[row][c] = 0.0f;
-    }
-    for (int i = lane; i < used; i += 32)
-#pragma unroll
-        for (int row = 0; row < ROWS; ++row)
-            if (row < owned) top[row] = fmaxf(top[row], __ldcg(partial + static_cast<long long>(i) * PIECE + row));
-#pragma unroll
-    for (int row = 0; row < ROWS; ++row)
-#pragma unroll
-        for (int step = 16; step > 0; step /= 2) top[row] = fmaxf(top[row], __shfl_xor_sync(0xffffffffu, top[row], step));
-#pragma unroll 2
-    for (int i = warp; i < used; i += DECODE_WARPS) {
-        const float *one = partial + static_cast<long long>(i) * PIECE;
-#pragma unroll
-        for (int row = 0; row < ROWS; ++row) {
-            if (row >= owned) break;
-            const float weight = exp2_fast(__ldcg(one + row) - (top[row] == -INFINITY ? 0.0f : top[row]));
-            total[row] = fmaf(__ldcg(one + ROWS + row), weight, total[row]);
-            float part[EACH];
-            if constexpr (EACH == 4) {
-                const float4 f = __ldcg(reinterpret_cast<const float4 *>(one + 2 * ROWS + row * DIM + lane * EACH));
-                part[0] = f.x, part[1] = f.y, part[2] = f.z, part[3] = f.w;
-            } else {
-                const float2 f = __ldcg(reinterpret_cast<const float2 *>(one + 2 * ROWS + row * DIM + lane * EACH));
-                part[0] = f.x, part[1] = f.y;
-            }
-#pragma unroll
-            for (int c = 0; c < EACH; ++c) sum[row][c] = fmaf(part[c], weight, sum[row][c]);
+            for (int c = 0; c < EACH; ++c) sum[r][c] = 0.0f;
         }
-    }
+        for (int i = lane; i < used; i += 32)
 #pragma unroll
-    for (int row = 0; row < ROWS; ++row) {
-        if (lane == 0) join_m[warp][row] = top[row], join_l[warp][row] = total[row];
+            for (int r = 0; r < AT_ONCE; ++r) top[r] = fmaxf(top[r], __ldcg(partial + static_cast<long long>(i) * PIECE + rows_of[r]));
 #pragma unroll
-        for (int c = 0; c < EACH; ++c) join_o[warp][row][lane * EACH + c] = sum[row][c];
+        for (int r = 0; r < AT_ONCE; ++r) {
+#pragma unroll
+            for (int step = 16; step > 0; step /= 2) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], step));
+        }
+#pragma unroll 4
+        for (int i = warp; i < used; i += DECODE_WARPS) {
+            const float *one = partial + static_cast<long long>(i) * PIECE;
+#pragma unroll
+            for (int r = 0; r < AT_ONCE; ++r) {
+                const int row = rows_of[r];
+                const float weight = exp2_fast(__ldcg(one + row) - (top[r] == -INFINITY ? 0.0f : top[r]));
+                total[r] = fmaf(__ldcg(one + ROWS + row), weight, total[r]);
+                float part[EACH];
+                if constexpr (EACH == 4) {
+                    const float4 f = __ldcg(reinterpret_cast<const float4 *>(one + 2 * ROWS + row * DIM + lane * EACH));
+                    part[0] = f.x, part[1] = f.y, part[2] = f.z, part[3] = f.w;
+                } else {
+                    const float2 f = __ldcg(reinterpret_cast<const float2 *>(one + 2 * ROWS + row * DIM + lane * EACH));
+                    part[0] = f.x, part[1] = f.y;
+                }
+#pragma unroll
+                for (int c = 0; c < EACH; ++c) sum[r][c] = fmaf(part[c], weight, sum[r][c]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) {
+            if (lane == 0) join_m[warp][rows_of[r]] = top[r], join_l[warp][rows_of[r]] = total[r];
+#pragma unroll
+            for (int c = 0; c < EACH; ++c) join_o[warp][rows_of[r]][lane * EACH + c] = sum[r][c];
+        }
     }
     __syncthreads();
     for (int item = threadIdx.x; item < owned * (DIM / 2); item += DECODE_THREADS) {

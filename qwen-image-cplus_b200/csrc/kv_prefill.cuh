@@ -28,8 +28,6 @@ namespace kv {
 constexpr int PREFILL_THREADS = 512, TILE_ROWS = 128, TILE_TOKENS = 128, PREFILL_ROWS = 2 * TILE_ROWS;
 constexpr int WIDEN_WARP0 = 8, ISSUE_WARP = 12, LOOK_UP_WARP = 13, TILE_BLOCKS = TILE_TOKENS / BLOCK, SLOTS = 4;
 constexpr int HALF_TOKENS = TILE_TOKENS / 2, HALF_BLOCKS = TILE_BLOCKS / 2;
-constexpr float PREFILL_SHIFT = 7.0f, MOST_OF_BLOCK = 32768.0f;
-constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
 constexpr uint32_t TMEM_S = 0, TMEM_O = 256;
 
 template <int DIM>
@@ -135,7 +133,7 @@ __device__ __forceinline__ void join_pieces(const Attention &a, const Entry &ent
             *reinterpret_cast<uint4 *>(a.y + out_row * a.ld_y + out_head * DIM + channel + 8 * half) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
         }
     }
-    if (a.lse != nullptr) a.lse[out_row * a.heads + out_head] = total == 0.0f ? -INFINITY : 0.6931471805599453f * (top - PREFILL_SHIFT + log2f(total));
+    if (a.lse != nullptr) a.lse[out_row * a.heads + out_head] = total == 0.0f ? -INFINITY : 0.6931471805599453f * (top - P_SHIFT + log2f(total));
 }
 
 template <int DIM>
@@ -316,8 +314,8 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     if (lane < TILE_BLOCKS) {
                         places[j % SLOTS][lane] = place;
                         scales[j % SLOTS][0][lane] = fmaxf(k_scale * a.scale_log2, LEAST_FACTOR);
-                        scales[j % SLOTS][1][lane] = log2f(v_scale);
-                        scales[j % SLOTS][2][lane] = __frcp_rn(v_scale);
+                        scales[j % SLOTS][1][lane] = log2_fast(v_scale);
+                        scales[j % SLOTS][2][lane] = reciprocal_fast(v_scale);
                     }
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(slot_full + j % SLOTS);
@@ -418,7 +416,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                     l *= shrink;
                                 }
                             }
-                            const float base = (m == -INFINITY ? 0.0f : m) - PREFILL_SHIFT;
+                            const float base = (m == -INFINITY ? 0.0f : m) - P_SHIFT;
                             float worst = 0.0f;
                             l_next = l;
                             ask(0);
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                 worst = fmaxf(worst, even + odd);
                                 l_next = fmaf(even + odd, factors[2][first + k], l_next);
                             }
-                            if (again || __all_sync(0xffffffffu, worst <= MOST_OF_BLOCK)) break;
+                            if (again || __all_sync(0xffffffffu, worst <= MOST_SUM)) break;
                             again = true;
                         }
                         if (!alive) break;
@@ -497,7 +495,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                         }
                     }
                     if (row < rows && used == 1) {
-                        if (a.lse != nullptr) a.lse[out_row * a.heads + out_head] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m - PREFILL_SHIFT + log2f(l));
+                        if (a.lse != nullptr) a.lse[out_row * a.heads + out_head] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m - P_SHIFT + log2f(l));
                     } else if (row < rows) {
                         partial[local] = m, partial[PREFILL_ROWS + local] = l;
                     }
