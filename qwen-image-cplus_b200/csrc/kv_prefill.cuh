@@ -374,13 +374,13 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                         const uint32_t half_at = s_at + h * HALF_TOKENS;
                         const float(*factors)[TILE_BLOCKS] = &scales[j % SLOTS][0];
                         const int first = h * HALF_BLOCKS;
-                        // the 16 scores of a block; the next block's are on their way meanwhile
-                        uint32_t s[2][BLOCK], p[32];
-                        auto ask = [&](int k) { tmem_load_32x16(half_at + k * BLOCK, s[k & 1]); };
-                        auto take = [&](int k) {
+                        uint32_t s[HALF_BLOCKS / 2][32], p[32];  // scores, weights in pairs
+                        auto take = [&]() {
+#pragma unroll
+                            for (int i = 0; i < HALF_BLOCKS / 2; ++i) tmem_load_32x32(half_at + i * 32, s[i]);
                             tmem_load_wait();
-                            arrived(s[k & 1]);
-                            if (k + 1 < HALF_BLOCKS) ask(k + 1);
+#pragma unroll
+                            for (int i = 0; i < HALF_BLOCKS / 2; ++i) arrived(s[i]);
                         };
                         float l_next;
                         bool again = __any_sync(0xffffffffu, m == -INFINITY);  // a row that has seen nothing yet
@@ -388,13 +388,12 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                         while (true) {
                             if (again) {  // the maximum of every row, so that none can be over it below
                                 float top = m;
-                                ask(0);
+                                take();
 #pragma unroll
                                 for (int k = 0; k < HALF_BLOCKS; ++k) {
-                                    take(k);
                                     float most = -INFINITY;
 #pragma unroll
-                                    for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k & 1][c]));
+                                    for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k / 2][k % 2 * BLOCK + c]));
                                     top = fmaxf(top, fmaf(most, factors[0][first + k], factors[1][first + k]));
                                 }
                                 const float shrink = m != -INFINITY ? exp2_fast(m - top) : 1.0f;
@@ -419,17 +418,16 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                             const float base = (m == -INFINITY ? 0.0f : m) - P_SHIFT;
                             float worst = 0.0f;
                             l_next = l;
-                            ask(0);
+                            take();
 #pragma unroll
                             for (int k = 0; k < HALF_BLOCKS; ++k) {
-                                take(k);
                                 const float factor = factors[0][first + k], offset = factors[1][first + k] - base;
                                 const uint64_t factor2 = pack_f32x2(factor, factor), offset2 = pack_f32x2(offset, offset);
                                 uint64_t sums = pack_f32x2(0.0f, 0.0f);
 #pragma unroll
                                 for (int c = 0; c < BLOCK; c += 2) {
                                     float low, high;
-                                    unpack_f32x2(fma_f32x2(pack_u32x2(s[k & 1][c], s[k & 1][c + 1]), factor2, offset2), low, high);
+                                    unpack_f32x2(fma_f32x2(pack_u32x2(s[k / 2][k % 2 * BLOCK + c], s[k / 2][k % 2 * BLOCK + c + 1]), factor2, offset2), low, high);
                                     low = exp2_fast(low), high = exp2_fast(high);
                                     sums = add_f32x2(sums, pack_f32x2(low, high));
                                     const __half2 pair = __floats2half2_rn(low, high);
