@@ -35,7 +35,7 @@ struct Prefill {
     static constexpr int HALVES = DIM / 64;                            // 128-byte rows of 64 channels
     static constexpr int OPERAND_BYTES = TILE_TOKENS * DIM * 2;        // of K, V, or half of Q
     static constexpr int Q_AT = 0, K_AT = 2 * OPERAND_BYTES, V_AT = 4 * OPERAND_BYTES, SCALES_AT = 6 * OPERAND_BYTES;
-    static constexpr int PLACES_AT = SCALES_AT + SLOTS * 3 * TILE_BLOCKS * 4, BARRIERS_AT = PLACES_AT + SLOTS * TILE_BLOCKS * 8;
+    static constexpr int PLACES_AT = SCALES_AT + SLOTS * TILE_BLOCKS * 16, BARRIERS_AT = PLACES_AT + SLOTS * TILE_BLOCKS * 8;
     static constexpr int BARRIERS = 8 + 2 * SLOTS + 10 + 1;
     static constexpr int SMEM_BYTES = BARRIERS_AT + BARRIERS * 8 + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     using P = Prefill<DIM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float(*scales)[3][TILE_BLOCKS] = reinterpret_cast<float(*)[3][TILE_BLOCKS]>(smem + P::SCALES_AT);  // factor, offset, 1 / sv of each block
-    long long(*places)[TILE_BLOCKS] = reinterpret_cast<long long(*)[TILE_BLOCKS]>(smem + P::PLACES_AT);  // its token row; -1: none
+    float4(*scales)[TILE_BLOCKS] = reinterpret_cast<float4(*)[TILE_BLOCKS]>(smem + P::SCALES_AT);  // factor, offset, 1 / sv of each block
+    long long(*places)[TILE_BLOCKS] = reinterpret_cast<long long(*)[TILE_BLOCKS]>(smem + P::PLACES_AT);  // its token row
     uint64_t *barriers = reinterpret_cast<uint64_t *>(smem + P::BARRIERS_AT);
     uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *slot_full = barriers + 8, *slot_empty = slot_full + SLOTS;
     uint64_t *s_full = slot_empty + SLOTS, *p_full = s_full + 2, *o_done = s_full + 6, *q_full = s_full + 10;  // of p and o [half of a tile][half of the rows]
@@ -192,35 +192,28 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
         if (warp >= WIDEN_WARP0 && warp < ISSUE_WARP) {
             // ---- codes ----
             setmaxnreg_dec<104>();
+            // A thread takes 16 codes of a token, the same ones of every TOKENS-th token. Eight threads that store together have four
+            // pieces of one 128-byte row and four of the next, so that they meet no bank twice.
             constexpr int LANES = DIM / 16, TOKENS = 128 / LANES, LOADS = TILE_TOKENS / TOKENS;  // threads to a token, tokens and loads of a pass
-            const int t = threadIdx.x - WIDEN_WARP0 * 32, row0 = t / LANES, chunk = t % LANES;
+            const int t = threadIdx.x - WIDEN_WARP0 * 32;
+            const int pair = t / (2 * LANES), row0 = pair * 2 + t / 4 % 2, chunk = t % 4 + t % (2 * LANES) / 8 * 4;
+            const uint32_t piece = chunk % 4 * 2, at0 = smem_u32(smem) + chunk / 4 * (TILE_TOKENS * 128) + row0 * 128;
+            const uint32_t first_at = at0 + ((piece ^ (row0 & 7)) << 4), second_at = at0 + (((piece + 1) ^ (row0 & 7)) << 4);
+            static_assert(TOKENS % 8 == 0, "a thread's rows have their last three bits in common");
+            const uint8_t *sources[2] = {cache.codes[0] + row0 % BLOCK * DIM + chunk * 16, cache.codes[1] + row0 % BLOCK * DIM + chunk * 16};
             uint4 words[2][LOADS];  // of keys, of values
             auto fetch = [&](int which, int j) {
+                const long long *place = places[j % SLOTS] + row0 / BLOCK;
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int token = i * TOKENS + row0;
-                    const long long place = j < tiles ? places[j % SLOTS][token / BLOCK] : -1;
-                    words[which][i] = place < 0 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u)
-                                                : load_codes(cache.codes[which] + (place + token % BLOCK) * DIM + chunk * 16);
-                }
+                for (int i = 0; i < LOADS; ++i) words[which][i] = load_codes(sources[which] + place[i * TOKENS / BLOCK] * DIM);
             };
-            auto widen = [&](int which, uint32_t base) {
-                // the two 16-byte pieces in the other order for every second half, so that eight threads meet no bank twice
-                const uint32_t half = chunk / 4, piece = chunk % 4 * 2, swap = half;
+            auto widen = [&](int which, uint32_t offset) {
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const uint32_t row = i * TOKENS + row0;
-                    const uint32_t w[4] = {words[which][i].x, words[which][i].y, words[which][i].z, words[which][i].w};
-                    uint32_t out[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) out[2 * k] = widen2<0x4140>(w[k]), out[2 * k + 1] = widen2<0x4342>(w[k]);
-                    const uint32_t at = base + half * (TILE_TOKENS * 128) + row * 128;
-#pragma unroll
-                    for (uint32_t k = 0; k < 2; ++k) {
-                        const uint32_t p = k ^ swap;
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((piece + p) ^ (row & 7)) << 4)), "r"(p ? out[4] : out[0]), "r"(p ? out[5] : out[1]),
-                                     "r"(p ? out[6] : out[2]), "r"(p ? out[7] : out[3]) : "memory");
-                    }
+                    const uint4 w = words[which][i];
+                    const uint32_t to = offset + i * (TOKENS * 128);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(first_at + to), "r"(widen2<0x4140>(w.x)), "r"(widen2<0x4342>(w.x)), "r"(widen2<0x4140>(w.y)), "r"(widen2<0x4342>(w.y)) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(second_at + to), "r"(widen2<0x4140>(w.z)), "r"(widen2<0x4342>(w.z)), "r"(widen2<0x4140>(w.w)), "r"(widen2<0x4342>(w.w)) : "memory");
                 }
             };
             bool alive = tiles > 0 && mbarrier_wait_warp(slot_full, 0, &g_status, STATUS_WAIT_FULL | 0xC020, lane);
@@ -228,14 +221,22 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             for (int j = 0; j < tiles && alive; ++j) {
                 const int stage = j & 1, phase = j >> 1 & 1;
                 if (!mbarrier_wait_warp(k_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC000 | stage, lane)) { alive = false; break; }
-                widen(0, smem_u32(smem + P::K_AT + stage * P::OPERAND_BYTES));
+                widen(0, P::K_AT + stage * P::OPERAND_BYTES);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbarrier_arrive(k_full + stage);
-                if (j + 1 < tiles && !mbarrier_wait_warp(slot_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
+                if (j + 1 == tiles) {
+                    if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) break;
+                    widen(1, P::V_AT + stage * P::OPERAND_BYTES);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbarrier_arrive(v_full + stage);
+                    break;
+                }
+                if (!mbarrier_wait_warp(slot_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
                 fetch(0, j + 1);
                 if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) { alive = false; break; }
-                widen(1, smem_u32(smem + P::V_AT + stage * P::OPERAND_BYTES));
+                widen(1, P::V_AT + stage * P::OPERAND_BYTES);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbarrier_arrive(v_full + stage);
@@ -304,18 +305,18 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                 for (int j = 0; j < tiles; ++j) {
                     const int next_page = page_at(j + 1), token = begin + j * TILE_TOKENS + lane * BLOCK;
                     if (page < 0 || page >= cache.pages) complain(0xC041), page = 0;
-                    long long place = -1;
+                    long long place = 0;
                     float k_scale = 0.0f, v_scale = 1.0f;
                     if (lane < TILE_BLOCKS && token < end) {
                         place = token_row(cache, page, head, token);
                         k_scale = __ldg(cache.scales[0] + place / BLOCK), v_scale = fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE);
                     }
+                    const long long first_place = __shfl_sync(0xffffffffu, place, 0);  // there is a token in the tile's first block
+                    if (token >= end) place = first_place;                             // what is fetched for nothing is masked, and finite
                     if (j >= SLOTS && !mbarrier_wait_warp(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, &g_status, STATUS_WAIT_EMPTY | 0xC240, lane)) break;
                     if (lane < TILE_BLOCKS) {
                         places[j % SLOTS][lane] = place;
-                        scales[j % SLOTS][0][lane] = fmaxf(k_scale * a.scale_log2, LEAST_FACTOR);
-                        scales[j % SLOTS][1][lane] = log2_fast(v_scale);
-                        scales[j % SLOTS][2][lane] = reciprocal_fast(v_scale);
+                        scales[j % SLOTS][lane] = make_float4(fmaxf(k_scale * a.scale_log2, LEAST_FACTOR), log2_fast(v_scale), reciprocal_fast(v_scale), 0.0f);
                     }
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(slot_full + j % SLOTS);
@@ -372,8 +373,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t half_at = s_at + h * HALF_TOKENS;
-                        const float(*factors)[TILE_BLOCKS] = &scales[j % SLOTS][0];
-                        const int first = h * HALF_BLOCKS;
+                        const float4 *scale = &scales[j % SLOTS][h * HALF_BLOCKS];
                         uint32_t s[HALF_BLOCKS / 2][32], p[32];  // scores, weights in pairs
                         auto take = [&]() {
 #pragma unroll
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                     float most = -INFINITY;
 #pragma unroll
                                     for (int c = 0; c < BLOCK; ++c) most = fmaxf(most, __uint_as_float(s[k / 2][k % 2 * BLOCK + c]));
-                                    top = fmaxf(top, fmaf(most, factors[0][first + k], factors[1][first + k]));
+                                    top = fmaxf(top, fmaf(most, scale[k].x, scale[k].y));
                                 }
                                 const float shrink = m != -INFINITY ? exp2_fast(m - top) : 1.0f;
                                 m = top;
@@ -421,7 +421,8 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                             take();
 #pragma unroll
                             for (int k = 0; k < HALF_BLOCKS; ++k) {
-                                const float factor = factors[0][first + k], offset = factors[1][first + k] - base;
+                                const float4 f = scale[k];
+                                const float factor = f.x, offset = f.y - base;
                                 const uint64_t factor2 = pack_f32x2(factor, factor), offset2 = pack_f32x2(offset, offset);
                                 uint64_t sums = pack_f32x2(0.0f, 0.0f);
 #pragma unroll
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                 float even, odd;
                                 unpack_f32x2(sums, even, odd);
                                 worst = fmaxf(worst, even + odd);
-                                l_next = fmaf(even + odd, factors[2][first + k], l_next);
+                                l_next = fmaf(even + odd, f.z, l_next);
                             }
                             if (again || __all_sync(0xffffffffu, worst <= MOST_SUM)) break;
                             again = true;
