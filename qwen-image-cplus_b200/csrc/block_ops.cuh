@@ -69,24 +69,28 @@ int launch_grid(void (*kernel)(Parameters...), dim3 grid, int threads, int smem_
     return static_cast<int>(launched(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...)));
 }
 
+// CTAs to an entry for the kernels that take a block of a head with each warp, of keys or of values; -1: too many.
+long long cache_grid(const qi_kv_cache *cache, const qi_kv_batch *batch) {
+    const long long blocks = (static_cast<long long>(batch->most) + 2 * kv::BLOCK - 2) / kv::BLOCK;  // that `most` tokens in a row can touch
+    const long long grid = (blocks * cache->kv_heads * 2 + kv::UNIT_WARPS - 1) / kv::UNIT_WARPS;
+    return grid > 0x7fffffff / kv::UNIT_WARPS ? -1 : grid;
+}
+
 template <typename T>
 int launch_append(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k, const void *v, long long ld_k, long long ld_v, void *stream) {
-    const long long blocks = (static_cast<long long>(batch->most) + 2 * kv::BLOCK - 2) / kv::BLOCK;  // that `most` tokens in a row can touch
-    const long long units = blocks * cache->kv_heads * 2;
-    const long long grid = (units + kv::APPEND_WARPS - 1) / kv::APPEND_WARPS;
-    if (grid > 0x7fffffff / kv::APPEND_WARPS) return INVALID;
+    const long long grid = cache_grid(cache, batch);
+    if (grid < 0) return INVALID;
     auto kernel = cache->head_dim == 128 ? kv::append_kernel<T, 128> : kv::append_kernel<T, 64>;
-    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::APPEND_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
+    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::UNIT_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
                        static_cast<const T *>(k), static_cast<const T *>(v), ld_k, ld_v);
 }
 
 template <typename T>
 int launch_read(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, void *k, void *v, long long ld_k, long long ld_v, void *stream) {
-    const long long quads = static_cast<long long>(batch->most) * cache->kv_heads * (cache->head_dim / 4), each = kv::READ_THREADS * kv::READ_ROWS;
-    const long long grid = (quads + each - 1) / each;
-    if (grid > 0x7fffffff) return INVALID;
+    const long long grid = cache_grid(cache, batch);
+    if (grid < 0) return INVALID;
     auto kernel = cache->head_dim == 128 ? kv::read_kernel<T, 128> : kv::read_kernel<T, 64>;
-    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries, 2), kv::READ_THREADS, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
+    return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::UNIT_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
                        static_cast<T *>(k), static_cast<T *>(v), ld_k, ld_v);
 }
 
@@ -143,6 +147,23 @@ int launch_prefill(const dim3 grid, const kv::Cache &cache, const kv::Tables &ta
     static std::atomic<bool> configured[MAX_DEVICES];
     if (const cudaError_t error = configure_once(kv::prefill_kernel<DIM>, kv::Prefill<DIM>::SMEM_BYTES, configured[device])) return static_cast<int>(error);
     return launch_grid(kv::prefill_kernel<DIM>, grid, kv::PREFILL_THREADS, kv::Prefill<DIM>::SMEM_BYTES, stream, cache, tables, batch, a);
+}
+
+// As many CTAs as run at once, each with its share of the rows: with twice as many, a last round left SMs idle.
+template <int THREADS, int PIECES>
+int launch_norm(const gated_norm::Arguments &a, void *stream) {
+    const int device = current_device();
+    if (device < 0) return static_cast<int>(cudaErrorNoDevice);
+    static std::atomic<int> cached[MAX_DEVICES];
+    int ctas = cached[device].load(std::memory_order_relaxed);
+    if (ctas == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, gated_norm::norm_kernel<THREADS, PIECES>, THREADS, 0) != cudaSuccess || ctas <= 0) {
+            (void)cudaGetLastError();
+            ctas = 1;
+        }
+        cached[device].store(ctas, std::memory_order_relaxed);
+    }
+    return launch_grid(gated_norm::norm_kernel<THREADS, PIECES>, dim3(std::min(a.rows, ctas * sm_count(device))), THREADS, 0, stream, a);
 }
 
 kv::PageTables page_tables_of(const qi_kv_cache *cache, const qi_kv_pages *pages) {
@@ -303,12 +324,11 @@ int qi_gated_norm_ex(const qi_gated_norm *call, void *stream) {
     a.residual_f16 = call->residual_dtype == QI_DTYPE_F16, a.branch_f16 = call->branch_dtype == QI_DTYPE_F16;
     a.vector_f16 = call->vector_dtype == QI_DTYPE_F16, a.y_f16 = call->y_dtype == QI_DTYPE_F16;
     a.branch_norm = call->branch_norm != 0, a.layer = call->kind == QI_NORM_LAYER;
-    const int most = sms_or_usual() * 8, grid = a.rows < most ? a.rows : most;
-    if (a.width <= 1024) return launch_grid(gated_norm::norm_kernel<128, 1>, dim3(grid), 128, 0, stream, a);
-    if (a.width <= 2048) return launch_grid(gated_norm::norm_kernel<256, 1>, dim3(grid), 256, 0, stream, a);
-    if (a.width <= 4096) return launch_grid(gated_norm::norm_kernel<256, 2>, dim3(grid), 256, 0, stream, a);
-    if (a.width <= 8192) return launch_grid(gated_norm::norm_kernel<512, 2>, dim3(grid), 512, 0, stream, a);
-    return launch_grid(gated_norm::norm_kernel<512, 4>, dim3(grid), 512, 0, stream, a);
+    if (a.width <= 1024) return launch_norm<128, 1>(a, stream);
+    if (a.width <= 2048) return launch_norm<256, 1>(a, stream);
+    if (a.width <= 4096) return launch_norm<256, 2>(a, stream);
+    if (a.width <= 8192) return launch_norm<512, 2>(a, stream);
+    return launch_norm<512, 4>(a, stream);
 }
 
 }  // extern "C"

@@ -5,8 +5,10 @@
 //
 // Each row is read once and written once; the values stay in registers between the sums, which are float32 and taken about the
 // mean (passes over registers, so that a large mean costs no digits). r' enters the second norm unrounded, also where it is
-// stored as float16. Bound by memory: THREADS threads hold a row, 8 adjacent values a piece, so that every access is 16 bytes a thread or
-// more. CTAs walk over rows; the vectors (gate, scale, shift, weights) then come from L1, past which the rows are streamed.
+// stored as float16. Bound by memory, and by what stands between a row's loads and its stores: up to four sums over the CTA. So each CTA
+// walks over its share of the rows with the next row's loads under way (three CTAs of 256 threads to an SM; 16384 rows of 4096: 156 us,
+// 5.2 TB/s; five CTAs without loads ahead 163, eight that do not all run at once 174). The vectors (gate, scale, shift, weights) come
+// from L1: a ring of rows in shared memory, filled by bulk copies, leaves no room for them there and took 203 us.
 #pragma once
 #include "ptx.cuh"
 
@@ -27,26 +29,34 @@ struct Arguments {
     bool residual_f16, branch_f16, vector_f16, y_f16, branch_norm, layer;
 };
 
-__device__ __forceinline__ void widen8(const uint4 w, float (&x)[8]) {
-    const uint32_t pairs[4] = {w.x, w.y, w.z, w.w};
+// Eight values from `at` on as they lie in memory: of a row, which are read once (STREAM), or of a vector, which other rows read too.
+struct Raw8 {
+    uint4 w[2];
+};
+template <bool STREAM>
+__device__ __forceinline__ void fetch8(const void *base, bool f16, long long at, Raw8 &raw) {
+    const uint4 *words = reinterpret_cast<const uint4 *>(static_cast<const char *>(base) + at * (f16 ? 2 : 4));
+    raw.w[0] = STREAM ? __ldcs(words) : __ldg(words);
+    if (!f16) raw.w[1] = STREAM ? __ldcs(words + 1) : __ldg(words + 1);
+}
+__device__ __forceinline__ void widen8(const Raw8 &raw, bool f16, float (&x)[8]) {
+    if (f16) {
+        const uint32_t pairs[4] = {raw.w[0].x, raw.w[0].y, raw.w[0].z, raw.w[0].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[j]));
-        x[2 * j] = f.x, x[2 * j + 1] = f.y;
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[j]));
+            x[2 * j] = f.x, x[2 * j + 1] = f.y;
+        }
+    } else {
+        const uint32_t words[8] = {raw.w[0].x, raw.w[0].y, raw.w[0].z, raw.w[0].w, raw.w[1].x, raw.w[1].y, raw.w[1].z, raw.w[1].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(words[j]);
     }
 }
-
-// Eight values from `at` on: a row's, which are read once (STREAM), or a vector's, which other rows read too.
-template <bool STREAM>
 __device__ __forceinline__ void load8(const void *base, bool f16, long long at, float (&x)[8]) {
-    if (f16) {
-        const uint4 *words = reinterpret_cast<const uint4 *>(static_cast<const __half *>(base) + at);
-        widen8(STREAM ? __ldcs(words) : __ldg(words), x);
-    } else {
-        const float4 *words = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-        const float4 a = STREAM ? __ldcs(words) : __ldg(words), b = STREAM ? __ldcs(words + 1) : __ldg(words + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    }
+    Raw8 raw;
+    fetch8<false>(base, f16, at, raw);
+    widen8(raw, f16, x);
 }
 
 __device__ __forceinline__ void store8(void *base, bool f16, long long at, const float (&x)[8]) {
@@ -81,7 +91,7 @@ __device__ __forceinline__ float2 block_sums(float2 value, float2 (&sums)[2][WAR
 }
 
 template <int THREADS, int PIECES>
-__global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
+__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 768 / THREADS : 1) norm_kernel(const Arguments a) {
     constexpr int WARPS = THREADS / 32;
     __shared__ float2 sums[2][WARPS];
     grid_wait();
@@ -116,19 +126,25 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
         shift_by(rest);
         return rsqrtf(fmaxf(fmaf(sum.y, per_value, -rest * rest), 0.0f) + a.epsilon);
     };
+    Raw8 raw_r[PIECES], raw_b[PIECES];  // the next row's values: on their way while this row's sums are waited for
+    auto fetch = [&](long long row) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int column = (p * THREADS + threadIdx.x) * 8;
+            raw_r[p].w[0] = raw_r[p].w[1] = raw_b[p].w[0] = raw_b[p].w[1] = make_uint4(0, 0, 0, 0);
+            if (row < a.rows && column < a.width) {
+                fetch8<true>(a.residual, a.residual_f16, row * a.width + column, raw_r[p]);
+                if (a.branch != nullptr) fetch8<true>(a.branch, a.branch_f16, row * a.width + column, raw_b[p]);
+            }
+        }
+    };
+    fetch(blockIdx.x);
     for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long start = static_cast<long long>(row) * a.width, vector = static_cast<long long>(row / a.rows_per_vector) * a.ld_vector;
         float r[PIECES][8], b[PIECES][8];
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int column = (p * THREADS + threadIdx.x) * 8;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) r[p][j] = b[p][j] = 0.0f;
-            if (column < a.width) {
-                load8<true>(a.residual, a.residual_f16, start + column, r[p]);
-                if (a.branch != nullptr) load8<true>(a.branch, a.branch_f16, start + column, b[p]);
-            }
-        }
+        for (int p = 0; p < PIECES; ++p) widen8(raw_r[p], a.residual_f16, r[p]), widen8(raw_b[p], a.branch_f16, b[p]);
+        fetch(static_cast<long long>(row) + gridDim.x);
         if (a.branch != nullptr) {
             const float factor = a.branch_norm ? normalise(b) : 1.0f;
 #pragma unroll
@@ -139,12 +155,12 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) b[p][j] *= factor;
                 if (a.branch_weight != nullptr) {
-                    load8<false>(a.branch_weight, false, column, v);
+                    load8(a.branch_weight, false, column, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
                 }
                 if (a.gate != nullptr) {
-                    load8<false>(a.gate, a.vector_f16, vector + column, v);
+                    load8(a.gate, a.vector_f16, vector + column, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
                 }
@@ -167,17 +183,17 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const Arguments a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) r[p][j] *= factor;
             if (a.weight != nullptr) {
-                load8<false>(a.weight, false, column, v);
+                load8(a.weight, false, column, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[p][j] *= v[j];
             }
             if (a.scale != nullptr) {
-                load8<false>(a.scale, a.vector_f16, vector + column, v);
+                load8(a.scale, a.vector_f16, vector + column, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[p][j] *= 1.0f + v[j];
             }
             if (a.shift != nullptr) {
-                load8<false>(a.shift, a.vector_f16, vector + column, v);
+                load8(a.shift, a.vector_f16, vector + column, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[p][j] += v[j];
             }

@@ -66,170 +66,163 @@ __device__ __forceinline__ long long token_row(const Cache &cache, int page, int
 // tokens, at least the scale that they have, and if it is more, they are rounded again: rint(code * (old / new)). New codes are
 // rint(value / scale). A block's scale never falls while it holds earlier tokens, so writing the same tokens again changes nothing.
 //
-// A warp takes one block of one head, of the keys or of the values: a lane holds 16 adjacent channels of every
-// (32 / (DIM / 16))-th token, so that codes leave in 16-byte pieces and the maximum is one reduction over the warp.
+// A warp takes one block of one head, of the keys or of the values: the maximum is one reduction over the warp, and a lane holds 16 bytes
+// of every (32 / (DIM / CHANNELS))-th token, so that loads and stores are whole lines. Bound by memory.
+//
+// rint(x / scale) is taken as x * (1 / scale), rounded by adding 1.5 * 2^23; the reciprocal is off by 2^-24 and the product by another, so a
+// quotient up to 127 is known to 2^-15, and a lane with one that near to a tie takes its eight or four again with the division. (With
+// divisions alone, 12 instructions each, 5700 tokens of 32 heads took 30 us more.)
 
-constexpr int APPEND_WARPS = 4;
+constexpr int UNIT_WARPS = 4;
 
-template <typename T, int DIM>
-__device__ __forceinline__ void load16(const T *source, float (&x)[16]) {
+// What one warp does: block `block` of the batch's entry, tokens [early, end) of it, and where its codes and its scale are.
+struct Unit {
+    Entry entry;
+    int which, head, block, start, early, end;
+    uint8_t *codes;  // of the block's first token
+    float *scale;
+};
+
+// False: nothing to do, or nothing that may be done.
+__device__ __forceinline__ bool read_unit(const Cache &cache, const Tables &tables, const Batch &batch, int dim, bool writes, uint32_t detail, Unit &u) {
+    const int lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * UNIT_WARPS + (threadIdx.x >> 5);  // (block, head, keys or values)
+    u.which = unit & 1, u.head = (unit >> 1) % cache.heads;
+    const bool sound = read_entry(batch, tables, cache.page_shift, blockIdx.y, 0x7fffffff, u.entry);
+    if (!sound || u.entry.count > u.entry.length) {
+        if (lane == 0) complain(detail);
+        return false;
+    }
+    u.start = u.entry.length - u.entry.count, u.block = u.start / BLOCK + (unit >> 1) / cache.heads;
+    const int first = u.block * BLOCK;
+    if (u.entry.count == 0 || first >= u.entry.length) return false;
+    const int page = __ldg(tables.table + static_cast<long long>(u.entry.slot) * tables.table_pages + (first >> cache.page_shift));
+    if (page < 0 || page >= cache.pages || (writes && __ldg(tables.references + page) != 1)) {  // no page, or one that others hold too
+        if (lane == 0) complain(detail + 1);
+        return false;
+    }
+    u.early = max(u.start - first, 0), u.end = min(u.entry.length - first, BLOCK);
+    const long long row = token_row(cache, page, u.head, first);
+    u.codes = (u.which == 0 ? cache.codes[0] : cache.codes[1]) + row * dim;
+    u.scale = (u.which == 0 ? cache.scales[0] : cache.scales[1]) + row / BLOCK;
+    return true;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_values(const T *source, float (&x)[16 / sizeof(T)]) {
     if constexpr (sizeof(T) == 2) {
-        const uint4 *words = reinterpret_cast<const uint4 *>(source);
+        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(source));
+        const uint32_t pairs[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 w = __ldg(words + i);
-            const uint32_t pairs[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[j]));
-                x[8 * i + 2 * j] = f.x, x[8 * i + 2 * j + 1] = f.y;
-            }
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[j]));
+            x[2 * j] = f.x, x[2 * j + 1] = f.y;
         }
     } else {
-        const float4 *words = reinterpret_cast<const float4 *>(source);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 w = __ldg(words + i);
-            x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
-        }
+        const float4 w = __ldg(reinterpret_cast<const float4 *>(source));
+        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
     }
 }
 
-// rint(x / scale) as a code, for |x| <= 127.5 * scale or so; a NaN becomes the code of zero.
-__device__ __forceinline__ uint32_t to_code(float x, float scale) {
-    const int code = __float2int_rn(__fdiv_rn(x, scale));
-    return static_cast<uint32_t>(min(max(code, -127), 127) + ZERO_CODE);
-}
+constexpr float ROUND_MAGIC = 12582912.0f, NEAR_TIE = 0.5f - 1.0f / 16384.0f, LEAST_NORMAL_SCALE = 1e-36f;
 
 template <typename T, int DIM>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(Cache cache, Tables tables, Batch batch, const T *k, const T *v, long long ld_k, long long ld_v) {
-    constexpr int LANES = DIM / 16, TOKENS = 32 / LANES, PASSES = BLOCK / TOKENS;  // lanes to a token, tokens and passes of a warp
+__global__ void __launch_bounds__(UNIT_WARPS * 32) append_kernel(Cache cache, Tables tables, Batch batch, const T *k, const T *v, long long ld_k, long long ld_v) {
+    constexpr int CHANNELS = 16 / sizeof(T), LANES = DIM / CHANNELS, TOKENS = 32 / LANES, PASSES = BLOCK / TOKENS;  // lanes to a token, tokens of a pass
     grid_wait();
     const int lane = threadIdx.x & 31;
-    const int unit = blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5);  // (block, head, keys or values)
-    const int which = unit & 1, head = (unit >> 1) % cache.heads, nth = (unit >> 1) / cache.heads;
-    Entry entry;
-    const bool sound = read_entry(batch, tables, cache.page_shift, blockIdx.y, 0x7fffffff, entry);
-    if (!sound || entry.count > entry.length) {
-        if (lane == 0) complain(0xC000);
-        return;
-    }
-    const int start = entry.length - entry.count, block = start / BLOCK + nth;
-    if (entry.count == 0 || block * BLOCK >= entry.length) return;
-    const int page = __ldg(tables.table + static_cast<long long>(entry.slot) * tables.table_pages + (block * BLOCK >> cache.page_shift));
-    if (page < 0 || page >= cache.pages || __ldg(tables.references + page) != 1) {  // no page, or one that others hold too
-        if (lane == 0) complain(0xC001);
-        return;
-    }
-    const int within = lane / LANES, channel = lane % LANES * 16;
-    const int early = max(start - block * BLOCK, 0), end = min(entry.length - block * BLOCK, BLOCK);  // tokens of the block: [early, end) are new
-    const T *source = (which == 0 ? k : v) + static_cast<long long>(head) * DIM + channel;
-    const long long ld = which == 0 ? ld_k : ld_v;
-    float x[PASSES][16];
+    Unit u;
+    if (!read_unit(cache, tables, batch, DIM, true, 0xC000, u)) return;
+    const int within = lane / LANES, channel = lane % LANES * CHANNELS;
+    const T *source = (u.which == 0 ? k : v) + static_cast<long long>(u.head) * DIM + channel;
+    const long long ld = u.which == 0 ? ld_k : ld_v, row0 = u.entry.first + static_cast<long long>(u.block) * BLOCK - u.start;
+    float x[PASSES][CHANNELS];
     float peak = 0.0f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int token = i * TOKENS + within;
-        if (token >= early && token < end) {
-            load16<T, DIM>(source + (entry.first + static_cast<long long>(block) * BLOCK + token - start) * ld, x[i]);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) peak = fmaxf(peak, fabsf(x[i][j]));
-        }
+        for (int j = 0; j < CHANNELS; ++j) x[i][j] = 0.0f;
+        if (token >= u.early && token < u.end) load_values(source + (row0 + token) * ld, x[i]);
     }
-    const long long row = token_row(cache, page, head, block * BLOCK);
-    uint8_t *codes = (which == 0 ? cache.codes[0] : cache.codes[1]) + row * DIM + channel;
-    float *held = (which == 0 ? cache.scales[0] : cache.scales[1]) + row / BLOCK;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int j = 0; j < CHANNELS; ++j) peak = fmaxf(peak, fabsf(x[i][j]));
     peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));  // no negative ones: ordered as whole numbers
-    const float old = early > 0 ? *held : 0.0f;
+    const float old = u.early > 0 ? *u.scale : 0.0f;
     const float scale = fmaxf(old, __fmul_rn(peak, 1.0f / 127.0f));
-    if (early > 0 && scale > old) {
+    if (u.early > 0 && scale > old) {
         const float factor = __fdiv_rn(old, scale);
+        for (int item = lane; item < u.early * (DIM / 4); item += 32) {
+            uint32_t *at = reinterpret_cast<uint32_t *>(u.codes) + item;
+            const uint32_t w = *at;
+            uint32_t out = 0;
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int token = i * TOKENS + within;
-            if (token >= early) continue;
-            uint4 *at = reinterpret_cast<uint4 *>(codes + token * DIM);
-            const uint4 w = *at;
-            uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t out = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int code = static_cast<int>(words[j] >> 8 * b & 255u) - ZERO_CODE;
-                    out |= static_cast<uint32_t>(__float2int_rn(static_cast<float>(code) * factor) + ZERO_CODE) << 8 * b;
-                }
-                words[j] = out;
+            for (int b = 0; b < 4; ++b) {
+                const int code = static_cast<int>(w >> 8 * b & 255u) - ZERO_CODE;
+                out |= static_cast<uint32_t>(__float2int_rn(static_cast<float>(code) * factor) + ZERO_CODE) << 8 * b;
             }
-            *at = make_uint4(words[0], words[1], words[2], words[3]);
+            *at = out;
         }
     }
+    const bool normal = scale >= LEAST_NORMAL_SCALE;
+    const float inverse = normal ? __frcp_rn(scale) : 0.0f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int token = i * TOKENS + within;
-        if (token < early || token >= end) continue;
-        uint32_t words[4];
+        if (token < u.early || token >= u.end) continue;
+        uint32_t bits[CHANNELS];
+        float furthest = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            words[j] = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) words[j] |= to_code(x[i][4 * j + b], scale) << 8 * b;
+        for (int j = 0; j < CHANNELS; ++j) {
+            const float q = x[i][j] * inverse, rounded = q + ROUND_MAGIC;
+            furthest = fmaxf(furthest, fabsf(q - (rounded - ROUND_MAGIC)));
+            bits[j] = __float_as_uint(rounded);
         }
-        *reinterpret_cast<uint4 *>(codes + token * DIM) = make_uint4(words[0], words[1], words[2], words[3]);
+        if (!(furthest < NEAR_TIE) || !normal) {
+#pragma unroll
+            for (int j = 0; j < CHANNELS; ++j) bits[j] = scale > 0.0f ? static_cast<uint32_t>(min(max(__float2int_rn(__fdiv_rn(x[i][j], scale)), -127), 127)) : 0u;
+        }
+        uint32_t words[CHANNELS / 4];
+#pragma unroll
+        for (int j = 0; j < CHANNELS / 4; ++j)  // the lowest bytes; two's complement becomes an offset of 128
+            words[j] = __byte_perm(__byte_perm(bits[4 * j], bits[4 * j + 1], 0x0040), __byte_perm(bits[4 * j + 2], bits[4 * j + 3], 0x0040), 0x5410) ^ 0x80808080u;
+        uint8_t *at = u.codes + token * DIM + channel;
+        if constexpr (CHANNELS == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(words[0], words[1]);
+        else *reinterpret_cast<uint32_t *>(at) = words[0];
     }
     __syncwarp();
-    if (lane == 0) *held = scale;
+    if (lane == 0) *u.scale = scale;
 }
 
 // ---- read back -----------------------------------------------------------------------------------------------------
 //
-// (code - 128) * scale of the last tokens of each entry, rounded once. A thread takes four adjacent channels, so that a warp
-// writes whole lines; ROWS tokens a thread keep enough loads in flight.
-
-constexpr int READ_THREADS = 256, READ_ROWS = 4;
+// (code - 128) * scale of the last tokens of each entry, rounded once. The same units as above; a lane takes four adjacent channels, so
+// that a warp writes whole lines.
 
 template <typename T, int DIM>
-__global__ void __launch_bounds__(READ_THREADS) read_kernel(Cache cache, Tables tables, Batch batch, T *k, T *v, long long ld_k, long long ld_v) {
+__global__ void __launch_bounds__(UNIT_WARPS * 32) read_kernel(Cache cache, Tables tables, Batch batch, T *k, T *v, long long ld_k, long long ld_v) {
+    constexpr int LANES = DIM / 4, TOKENS = 32 / LANES, PASSES = BLOCK / TOKENS;
     grid_wait();
-    Entry entry;
-    const bool sound = read_entry(batch, tables, cache.page_shift, blockIdx.y, 0x7fffffff, entry);
-    if (!sound || entry.count > entry.length) {
-        if (threadIdx.x == 0) complain(0xC010);
-        return;
-    }
-    constexpr int QUADS = DIM / 4;
-    const int row_quads = cache.heads * QUADS;
-    const int which = blockIdx.z;
-    T *out = which == 0 ? k : v;
-    const long long ld = which == 0 ? ld_k : ld_v, total = static_cast<long long>(entry.count) * row_quads;
-    const long long begin = static_cast<long long>(blockIdx.x) * (READ_THREADS * READ_ROWS) + threadIdx.x;
-    const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
-    uint32_t words[READ_ROWS];
-    float scales[READ_ROWS];
+    const int lane = threadIdx.x & 31;
+    Unit u;
+    if (!read_unit(cache, tables, batch, DIM, false, 0xC010, u)) return;
+    const int within = lane / LANES, channel = lane % LANES * 4;
+    const float scale = *u.scale;
+    uint32_t words[PASSES];
 #pragma unroll
-    for (int i = 0; i < READ_ROWS; ++i) {
-        const long long item = begin + i * READ_THREADS;
-        words[i] = 0x80808080u, scales[i] = 0.0f;
-        if (item >= total) continue;
-        const int t = static_cast<int>(item / row_quads), rest = static_cast<int>(item % row_quads), head = rest / QUADS;
-        const int token = entry.length - entry.count + t;
-        const int page = __ldg(pages + (token >> cache.page_shift));
-        if (page < 0 || page >= cache.pages) {
-            complain(0xC011);
-            continue;
-        }
-        const long long row = token_row(cache, page, head, token);
-        words[i] = *reinterpret_cast<const uint32_t *>((which == 0 ? cache.codes[0] : cache.codes[1]) + row * DIM + rest % QUADS * 4);
-        scales[i] = (which == 0 ? cache.scales[0] : cache.scales[1])[row / BLOCK];
-    }
+    for (int i = 0; i < PASSES; ++i) words[i] = *reinterpret_cast<const uint32_t *>(u.codes + (i * TOKENS + within) * DIM + channel);
+    const long long ld = u.which == 0 ? ld_k : ld_v, row0 = u.entry.first + static_cast<long long>(u.block) * BLOCK - u.start;
+    T *out = (u.which == 0 ? k : v) + static_cast<long long>(u.head) * DIM + channel;
 #pragma unroll
-    for (int i = 0; i < READ_ROWS; ++i) {
-        const long long item = begin + i * READ_THREADS;
-        if (item >= total) continue;
+    for (int i = 0; i < PASSES; ++i) {
+        const int token = i * TOKENS + within;
+        if (token < u.early || token >= u.end) continue;
         float x[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = static_cast<float>(static_cast<int>(words[i] >> 8 * b & 255u) - ZERO_CODE) * scales[i];
-        T *at = out + (entry.first + item / row_quads) * ld + item % row_quads * 4;
+        for (int b = 0; b < 4; ++b) x[b] = static_cast<float>(static_cast<int>(words[i] >> 8 * b & 255u) - ZERO_CODE) * scale;
+        T *at = out + (row0 + token) * ld;
         if constexpr (sizeof(T) == 4) {
             *reinterpret_cast<float4 *>(at) = make_float4(x[0], x[1], x[2], x[3]);
         } else {
