@@ -98,36 +98,41 @@ int launch_read(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_
 
 struct AttentionPlan {
     int tiles;  // of 8 query rows on mma.sync; 0: of 256 on tcgen05
-    int rows, row_tiles, chunk, splits;
+    int grid;   // of the former
+    int row_tiles, chunk, splits;
     size_t partial_offset, bytes;
 };
 
 constexpr int DECODE_ROWS = 16;  // query rows to a sequence and head of the cache up to which a CTA of the streaming kernel holds all
 
-// How a call is cut: query rows into tiles, and the tokens of a tile into pieces where there are too few tiles for the GPU.
+// How a call is cut. The streaming kernel shares the tokens out by itself. The other one takes a CTA to a tile of rows, one to an SM, and
+// where there are too few tiles for the GPU, several to pieces of its tokens.
 bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int window, int sms, AttentionPlan &plan) {
     if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
-    const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads);
+    const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads), entries = batch->entries > 0 ? batch->entries : 1;
     plan.tiles = rows <= 8 ? 1 : rows <= DECODE_ROWS ? 2 : 0;
-    plan.rows = plan.tiles > 0 ? 8 * plan.tiles : kv::PREFILL_ROWS;
-    const long long row_tiles = rows > 0 ? (rows + plan.rows - 1) / plan.rows : 1;
+    plan.grid = 2 * sms, plan.row_tiles = 1, plan.chunk = 0, plan.splits = 1;
+    if (plan.tiles > 0) {
+        plan.partial_offset = (static_cast<size_t>(entries) * cache->kv_heads * 4 + 255) / 256 * 256;
+        // units of one round each are never shared
+        plan.bytes = max_length <= kv::ROUND ? 0 : plan.partial_offset + static_cast<size_t>(plan.grid) * 2 * (8 * plan.tiles) * (cache->head_dim + 2) * 4;
+        return true;
+    }
+    const long long row_tiles = (rows + kv::PREFILL_ROWS - 1) / kv::PREFILL_ROWS;
     if (row_tiles * cache->kv_heads > 65535) return false;
     plan.row_tiles = static_cast<int>(row_tiles);
-    const long long units = row_tiles * cache->kv_heads * (batch->entries > 0 ? batch->entries : 1);
+    const long long units = row_tiles * cache->kv_heads * entries;
     long long span = max_length;  // of the tokens that a tile can see
     if (window > 0 && static_cast<long long>(window) + batch->most + kv::BLOCK < span) span = static_cast<long long>(window) + batch->most + kv::BLOCK;
-    // Pieces: streaming CTAs are small and many of them run at once; of the others one fills an SM, and pieces pay only while SMs are idle
-    const long long round = plan.tiles > 0 ? kv::DECODE_WARPS * kv::STEP : kv::TILE_TOKENS;
-    const long long pieces = plan.tiles > 0 ? (2LL * sms + units - 1) / units : sms / units > 1 ? sms / units : 1;
+    const long long pieces = sms / units > 1 ? sms / units : 1;
     long long chunk = (span + pieces - 1) / pieces;
-    chunk = (chunk + round - 1) / round * round;
-    if (chunk < round) chunk = round;
-    const long long splits = span > 0 ? (span + chunk - 1) / chunk : 1;
-    plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(splits);
+    chunk = (chunk + kv::TILE_TOKENS - 1) / kv::TILE_TOKENS * kv::TILE_TOKENS;
+    if (chunk < kv::TILE_TOKENS) chunk = kv::TILE_TOKENS;
+    plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(span > 0 ? (span + chunk - 1) / chunk : 1);
     plan.partial_offset = (static_cast<size_t>(units) * 4 + 255) / 256 * 256;
     // room for as many pieces as any window gives
-    const long long most = std::min(pieces, (max_length + round - 1) / round);
-    plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * plan.rows * (cache->head_dim + 2) * 4 : 0;
+    const long long most = std::min(pieces, (max_length + kv::TILE_TOKENS - 1LL) / kv::TILE_TOKENS);
+    plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * kv::PREFILL_ROWS * (cache->head_dim + 2) * 4 : 0;
     return true;
 }
 
@@ -248,7 +253,7 @@ int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const
     a.chunk = plan.chunk, a.splits = plan.splits, a.row_tiles = plan.row_tiles;
     a.arrivals = static_cast<int *>(workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.partial_offset);
-    const dim3 grid(plan.splits, cache->kv_heads * plan.row_tiles, batch->entries);
+    const dim3 grid = plan.tiles > 0 ? dim3(plan.grid) : dim3(plan.splits, cache->kv_heads * plan.row_tiles, batch->entries);
     if (plan.tiles == 0)
         return cache->head_dim == 128 ? launch_prefill<128>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream)
                                       : launch_prefill<64>(grid, layer_of(cache, call->layer), tables_of(pages), batch_of(batch), a, stream);

@@ -2,9 +2,12 @@
 //
 //   y_i = sum_j softmax_j(scale * q_i . k_j) v_j       k_j = (c_j - 128) * sk, v_j = (d_j - 128) * sv, sk and sv one for 16 tokens
 //
-// A CTA takes up to 8 * TILES query rows that share a head of the cache (group heads times tokens) and a piece of that head's
-// tokens. Each of its warps walks over steps of 32 tokens with sums of its own; warps are joined in shared memory, pieces in
-// a workspace, where the CTA that arrives last adds them up in their order (the same bits whichever is last).
+// The work is a list of rounds of 128 tokens: those of each unit (an entry and a head of the cache, with up to 8 * TILES query rows: group
+// heads times tokens) one after the other, unit after unit. Two CTAs an SM share it evenly, whatever the lengths, so that all end together
+// and each pays only once for its start; a ring of copies runs on from one unit into the next. A CTA's warps take 32 tokens of a round each,
+// with sums of their own; warps are joined in shared memory, and a unit that several CTAs share in a workspace, where the CTA that
+// arrives last adds the pieces up in their order (the same bits whichever is last). 64 sequences of 2048 to 8192 tokens, 8 heads, 131071
+// tokens of one: XX us, YY us; with a CTA to each piece of a unit 143 and 58.
 //
 // The products run transposed on m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an instruction are tokens and channels
 // of the cache, of which there are always enough, and the 8 columns are queries, of which there may be one. Which channel or
@@ -27,7 +30,7 @@ namespace kv {
 
 constexpr float P_SHIFT = 7.0f, MOST_SUM = 32768.0f, LEAST_SCALE = 8.6736174e-19f;  // 2^-60
 constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
-constexpr int DECODE_WARPS = 4, DECODE_THREADS = DECODE_WARPS * 32, STEP = 32;
+constexpr int DECODE_WARPS = 4, DECODE_THREADS = DECODE_WARPS * 32, STEP = 32, ROUND = DECODE_WARPS * STEP, LEAST_ROUNDS = 4;
 
 struct Attention {
     const __half *q;
@@ -37,9 +40,9 @@ struct Attention {
     int heads, group;   // query heads, and how many of them share a head of the cache
     float scale_log2;
     int causal, window, max_length;
-    int chunk, splits, row_tiles;
-    int *arrivals;      // [entries][kv_heads][row_tiles], zero between calls
-    float *partial;     // [entries][kv_heads][row_tiles][splits][rows][head_dim + 2]
+    int chunk, splits, row_tiles;  // of the kernel for many queries
+    int *arrivals;      // one for each unit or tile of rows, zero between calls
+    float *partial;     // what pieces leave: [piece][rows][head_dim + 2]
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -94,10 +97,10 @@ template <int DIM, int TILES>
 struct Decode {
     static constexpr int STAGES = DIM == 128 ? 3 : 5, STAGE_BYTES = 2 * STEP * DIM + 32;  // codes of keys, of values, scales
     struct Join {
-        float o[DECODE_WARPS][8 * TILES][DIM + 4], m[DECODE_WARPS][8 * TILES], l[DECODE_WARPS][8 * TILES];
+        float o[DECODE_WARPS][8 * TILES][DIM], m[DECODE_WARPS][8 * TILES], l[DECODE_WARPS][8 * TILES];
     };
-    static constexpr int SMEM_BYTES = DECODE_WARPS * STAGES * STAGE_BYTES;
-    static_assert(sizeof(Join) <= SMEM_BYTES, "warps are joined where their rings were");
+    static constexpr int JOIN_AT = DECODE_WARPS * STAGES * STAGE_BYTES, SMEM_BYTES = JOIN_AT + sizeof(Join);
+    static_assert(TILES > 1 || 2 * (SMEM_BYTES + 1024 + 256) <= 228 * 1024, "two CTAs to an SM");
 };
 
 // Where piece `piece` (16 bytes) of a token's codes lies in its row: keys are read by lanes of two tokens in turn with four pieces each, values
@@ -112,80 +115,113 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
     constexpr int ROWS = 8 * TILES, K_WORDS = DIM / 16;            // K_WORDS: 32-bit words of a token's codes that a lane holds (keys)
     constexpr int V_WORDS = DIM / 32, BLOCKS = STEP / BLOCK;       // and of values, of each of four tokens
     constexpr int STAGES = Decode<DIM, TILES>::STAGES, STAGE_BYTES = Decode<DIM, TILES>::STAGE_BYTES;
-    extern __shared__ uint8_t smem[];
+    constexpr int PIECE = ROWS * (DIM + 2);                        // floats that a CTA leaves of a unit it shares
+    extern __shared__ __align__(16) uint8_t smem[];
     using Join = typename Decode<DIM, TILES>::Join;
-    auto &join_o = reinterpret_cast<Join *>(smem)->o;
-    auto &join_m = reinterpret_cast<Join *>(smem)->m, &join_l = reinterpret_cast<Join *>(smem)->l;
-    __shared__ int is_last;
+    Join *join = reinterpret_cast<Join *>(smem + Decode<DIM, TILES>::JOIN_AT);
+    auto &join_o = join->o;
+    auto &join_m = join->m, &join_l = join->l;
+    __shared__ int is_last, first_entry;
+    __shared__ long long warp_rounds[DECODE_WARPS], warp_units[DECODE_WARPS], first_before;
     grid_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row8 = lane >> 2, quad = lane & 3;
-    const int split = blockIdx.x, head = blockIdx.y / a.row_tiles, tile = blockIdx.y % a.row_tiles, b = blockIdx.z;
-    Entry entry;
-    if (!read_entry(batch, tables, cache.page_shift, b, a.max_length, entry)) {
-        if (threadIdx.x == 0) complain(0xC030);
-        return;
-    }
-    const int rows = entry.count * a.group, first_row = tile * ROWS;
-    if (first_row >= rows) return;
-    const int last_row = min(first_row + ROWS, rows) - 1;
-    int low, high, unused;
-    visible(a, entry, first_row, low, unused);
-    visible(a, entry, last_row, unused, high);
-    low = low / BLOCK * BLOCK;
-    const int span = max(high - low, 0), used = max((span + a.chunk - 1) / a.chunk, 1);
-    if (split >= used) return;
-    const int begin = low + split * a.chunk, end = min(begin + a.chunk, high);  // this CTA's tokens
 
-    uint32_t q[TILES][K_WORDS][2];
-    int row_low[TILES][2], row_high[TILES][2];  // of this lane's columns of S^T
-    int all_low = 0, all_high = 0x7fffffff;     // what every row sees
-#pragma unroll
-    for (int n = 0; n < TILES; ++n) {
-        const int row = first_row + n * 8 + row8;
-        const __half *source = a.q + (entry.first + static_cast<long long>(row / a.group)) * a.ld_q + (head * a.group + row % a.group) * DIM;
-#pragma unroll
-        for (int j = 0; j < DIM / 64; ++j) {
-            uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-            if (row < rows) {
-                const uint4 *at = reinterpret_cast<const uint4 *>(source + (quad + 4 * j) * 16);
-                w[0] = __ldg(at), w[1] = __ldg(at + 1);
-            }
-            q[n][4 * j][0] = w[0].x, q[n][4 * j][1] = w[0].y, q[n][4 * j + 1][0] = w[0].z, q[n][4 * j + 1][1] = w[0].w;
-            q[n][4 * j + 2][0] = w[1].x, q[n][4 * j + 2][1] = w[1].y, q[n][4 * j + 3][0] = w[1].z, q[n][4 * j + 3][1] = w[1].w;
+    // ---- which rounds are this CTA's ----
+    struct Span {
+        Entry entry;
+        int low, high, rounds;  // the tokens that any row sees, low a multiple of 16; their rounds, at least one where there are rows
+    };
+    auto span_of = [&](int b, Span &u) {
+        u.rounds = 0, u.low = 0, u.high = 0;
+        if (!read_entry(batch, tables, cache.page_shift, b, a.max_length, u.entry)) {
+            complain(0xC030);
+            return;
         }
+        if (u.entry.count == 0) return;
+        int unused;
+        visible(a, u.entry, 0, u.low, unused);
+        visible(a, u.entry, u.entry.count * a.group - 1, unused, u.high);
+        u.low = u.low / BLOCK * BLOCK;
+        u.rounds = max((max(u.high - u.low, 0) + ROUND - 1) / ROUND, 1);
+    };
+    const int each = (batch.entries + DECODE_THREADS - 1) / DECODE_THREADS, from = threadIdx.x * each, to = min(from + each, batch.entries);
+    long long mine = 0, units = 0;
+    Span found;
+    for (int b = from; b < to; ++b) span_of(b, found), mine += found.rounds, units += found.rounds > 0;
+    long long before = mine;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) visible(a, entry, min(first_row + n * 8 + quad * 2 + i, last_row), row_low[n][i], row_high[n][i]);
+    for (int step = 1; step < 32; step *= 2) {
+        const long long below = __shfl_up_sync(0xffffffffu, before, step);
+        if (lane >= step) before += below;
+        units += __shfl_xor_sync(0xffffffffu, units, step);
     }
-    visible(a, entry, last_row, all_low, unused);
-    visible(a, entry, first_row, unused, all_high);
-
-    float o[TILES][DIM / 16][4], m[TILES][2], l[TILES][2];
+    if (lane == 31) warp_rounds[warp] = before, warp_units[warp] = units;
+    __syncthreads();
+    before -= mine;
+    long long total = 0;
+    units = 0;
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) {
-        m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DIM / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
+    for (int w = 0; w < DECODE_WARPS; ++w) {
+        if (w < warp) before += warp_rounds[w];
+        total += warp_rounds[w], units += warp_units[w];
     }
+    total *= cache.heads, units *= cache.heads;
+    if (total == 0) return;
+    // no more CTAs than have LEAST_ROUNDS each, or a unit: joining pieces costs as much as some rounds do
+    const long long wanted = max((total + LEAST_ROUNDS - 1) / LEAST_ROUNDS, units);
+    const long long ctas = min(static_cast<long long>(gridDim.x), wanted);
+    if (blockIdx.x >= ctas) return;
+    const long long first_round = blockIdx.x * total / ctas, end_round = (blockIdx.x + 1) * total / ctas;
+    auto cta_of = [&](long long round) { return ((round + 1) * ctas - 1) / total; };
+    if (mine > 0 && before * cache.heads <= first_round && first_round < (before + mine) * cache.heads) {
+        int b = from;
+        for (span_of(b, found); (before + found.rounds) * cache.heads <= first_round && b + 1 < to; span_of(++b, found)) before += found.rounds;
+        first_entry = b, first_before = before;
+    }
+    __syncthreads();
+    int b = first_entry;
+    long long unit_round = first_before * cache.heads;  // the first round of the unit
+    Span span;
+    span_of(b, span);
+    if (span.rounds == 0) return;
+    int head = static_cast<int>((first_round - unit_round) / span.rounds), r = static_cast<int>((first_round - unit_round) % span.rounds);
+    unit_round += static_cast<long long>(head) * span.rounds;
 
-    const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
     // Each warp has a ring of STAGES steps of its own in shared memory, filled by 16-byte asynchronous copies, 16 KB of them under way at
     // any time. Pieces of a row are stored where eight lanes that read together meet no bank twice (DIM 64, values: two of them do).
     uint8_t *ring = smem + warp * (STAGES * STAGE_BYTES);
-    auto place_of = [&](int token) -> long long {  // token row of a block; -1: none
-        if (token >= end) return -1;
-        int page = __ldg(pages + (token >> cache.page_shift));
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.pages)) complain(0xC031), page = 0;
-        return token_row(cache, page, head, token);
-    };
-    const bool one_page = cache.page_shift >= 5 && begin % STEP == 0;  // a step's blocks follow each other in memory
-    long long place[BLOCKS];                                           // of the step that is fetched next
-    auto look_up = [&](int token) {
+    // what is fetched next: it runs STAGES - 1 rounds ahead
+    Span ahead = span;
+    int ahead_entry = b, ahead_head = head, ahead_round = r;
+    long long left = end_round - first_round;
+    long long place[BLOCKS];  // token rows of its blocks; -1: none
+    auto look_up = [&]() {
+        const int token = ahead.low + ahead_round * ROUND + warp * STEP;
+        const int *pages = tables.table + static_cast<long long>(ahead.entry.slot) * tables.table_pages;
+        auto place_of = [&](int token) -> long long {
+            if (left <= 0 || token >= ahead.high) return -1;
+            int page = __ldg(pages + (token >> cache.page_shift));
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.pages)) complain(0xC031), page = 0;
+            return token_row(cache, page, ahead_head, token);
+        };
         place[0] = place_of(token);
-        if (one_page) place[1] = token + BLOCK < end ? place[0] + BLOCK : -1;
+        if (cache.page_shift >= 5 && ahead.low % STEP == 0) place[1] = place[0] >= 0 && token + BLOCK < ahead.high ? place[0] + BLOCK : -1;  // in the same page
         else place[1] = place_of(token + BLOCK);
     };
     static_assert(BLOCKS == 2, "look_up");
-    auto fetch = [&](int step) {  // the step's codes and scales, from `place`
+    auto go_on = [&]() {
+        --left;
+        if (++ahead_round == ahead.rounds && left > 0) {
+            ahead_round = 0;
+            if (++ahead_head == cache.heads) {
+                ahead_head = 0;
+                do span_of(++ahead_entry, ahead);
+                while (ahead.rounds == 0 && ahead_entry + 1 < batch.entries);
+            }
+        }
+        look_up();
+    };
+    auto fetch = [&](int step) {  // the round's codes and scales, from `place`
         uint8_t *stage = ring + step % STAGES * STAGE_BYTES;
 #pragma unroll
         for (int k = 0; k < BLOCKS; ++k) {
@@ -203,260 +239,309 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
         }
         cp_async_commit();
     };
-
-    int token = begin + warp * STEP;
-    look_up(token);
+    look_up();
     for (int step = 0; step < STAGES - 1; ++step) {
         fetch(step);
-        look_up(token + (step + 1) * DECODE_THREADS);
+        go_on();
     }
     int step = 0;
-    for (; token < end; token += DECODE_THREADS, ++step) {
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();  // the step is there for every lane, and the one before it is done with
-        fetch(step + STAGES - 1);
-        look_up(token + STAGES * DECODE_THREADS);
-        const uint8_t *stage = ring + step % STAGES * STAGE_BYTES;
-        float s[TILES][BLOCKS][4];
+    for (long long round = first_round; round < end_round;) {
+        // ---- one unit ----
+        const Entry &entry = span.entry;
+        const int rows = entry.count * a.group, end = span.high;
+        const int first = r, last = static_cast<int>(min(static_cast<long long>(span.rounds), r + end_round - round));  // rounds of it that are this CTA's
+        uint32_t q[TILES][K_WORDS][2];
+        int row_low[TILES][2], row_high[TILES][2];  // of this lane's columns of S^T
+        int all_low, all_high, unused;              // what every row sees
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
+        for (int n = 0; n < TILES; ++n) {
+            const int row = n * 8 + row8;
+            const __half *source = a.q + (entry.first + static_cast<long long>(row / a.group)) * a.ld_q + (head * a.group + row % a.group) * DIM;
 #pragma unroll
-            for (int n = 0; n < TILES; ++n) s[n][k][0] = s[n][k][1] = s[n][k][2] = s[n][k][3] = 0.0f;
-            uint32_t key[2][K_WORDS];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < DIM / 64; ++j) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + (k * BLOCK + row8 + 8 * i) * DIM + key_place<DIM>(row8, quad + 4 * j) * 16);
-                    key[i][4 * j] = w.x, key[i][4 * j + 1] = w.y, key[i][4 * j + 2] = w.z, key[i][4 * j + 3] = w.w;
+            for (int j = 0; j < DIM / 64; ++j) {
+                uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                if (row < rows) {
+                    const uint4 *at = reinterpret_cast<const uint4 *>(source + (quad + 4 * j) * 16);
+                    w[0] = __ldg(at), w[1] = __ldg(at + 1);
                 }
-#pragma unroll
-            for (int j = 0; j < K_WORDS; ++j) {
-                const uint32_t a0 = widen2<0x4140>(key[0][j]), a1 = widen2<0x4140>(key[1][j]), a2 = widen2<0x4342>(key[0][j]), a3 = widen2<0x4342>(key[1][j]);
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) mma_16x8x16(s[n][k], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
+                q[n][4 * j][0] = w[0].x, q[n][4 * j][1] = w[0].y, q[n][4 * j + 1][0] = w[0].z, q[n][4 * j + 1][1] = w[0].w;
+                q[n][4 * j + 2][0] = w[1].x, q[n][4 * j + 2][1] = w[1].y, q[n][4 * j + 3][0] = w[1].z, q[n][4 * j + 3][1] = w[1].w;
             }
-        }
-        float factor[BLOCKS], offset[BLOCKS], inverse[BLOCKS];
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            const float2 scales = *reinterpret_cast<const float2 *>(stage + 2 * STEP * DIM + 8 * k);
-            const bool there = token + k * BLOCK < end;
-            const float scale = there ? fmaxf(scales.y, LEAST_SCALE) : 1.0f;
-            factor[k] = there ? scales.x * a.scale_log2 : 0.0f, offset[k] = log2_fast(scale), inverse[k] = reciprocal_fast(scale);
+            for (int i = 0; i < 2; ++i) visible(a, entry, min(n * 8 + quad * 2 + i, rows - 1), row_low[n][i], row_high[n][i]);
         }
-        if (!(token >= all_low && token + STEP <= min(all_high, end))) {
-            // what is hidden: its score becomes -infinity, and the block's factor, if it is 0, something that leaves it that
+        visible(a, entry, rows - 1, all_low, unused);
+        visible(a, entry, 0, unused, all_high);
+        float o[TILES][DIM / 16][4], m[TILES][2], l[TILES][2];
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < DIM / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
+        }
+        for (; r < last; ++r, ++round, ++step) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();  // the round is there for every lane, and the one before it is done with
+            fetch(step + STAGES - 1);
+            go_on();
+            const int token = span.low + r * ROUND + warp * STEP;
+            if (token >= end) continue;
+            const uint8_t *stage = ring + step % STAGES * STAGE_BYTES;
+            float s[TILES][BLOCKS][4];
 #pragma unroll
             for (int k = 0; k < BLOCKS; ++k) {
-                factor[k] = fmaxf(factor[k], LEAST_FACTOR);
 #pragma unroll
-                for (int n = 0; n < TILES; ++n)
+                for (int n = 0; n < TILES; ++n) s[n][k][0] = s[n][k][1] = s[n][k][2] = s[n][k][3] = 0.0f;
+                uint32_t key[2][K_WORDS];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = token + k * BLOCK + row8 + i / 2 * 8;
-                        if (at < row_low[n][i & 1] || at >= min(row_high[n][i & 1], end)) s[n][k][i] = -INFINITY;
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < DIM / 64; ++j) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(stage + (k * BLOCK + row8 + 8 * i) * DIM + key_place<DIM>(row8, quad + 4 * j) * 16);
+                        key[i][4 * j] = w.x, key[i][4 * j + 1] = w.y, key[i][4 * j + 2] = w.z, key[i][4 * j + 3] = w.w;
                     }
-            }
-        }
-        float weight[TILES][BLOCKS][4], l_next[TILES][2];
-        bool nothing = false;  // a row that has seen nothing yet
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) nothing |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
-        bool again = __any_sync(0xffffffffu, nothing);
-        while (true) {
-            if (again) {
+                for (int j = 0; j < K_WORDS; ++j) {
+                    const uint32_t a0 = widen2<0x4140>(key[0][j]), a1 = widen2<0x4140>(key[1][j]), a2 = widen2<0x4342>(key[0][j]), a3 = widen2<0x4342>(key[1][j]);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) mma_16x8x16(s[n][k], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
+                }
+            }
+            float factor[BLOCKS], offset[BLOCKS], inverse[BLOCKS];
+#pragma unroll
+            for (int k = 0; k < BLOCKS; ++k) {
+                const float2 scales = *reinterpret_cast<const float2 *>(stage + 2 * STEP * DIM + 8 * k);
+                const bool there = token + k * BLOCK < end;
+                const float scale = there ? fmaxf(scales.y, LEAST_SCALE) : 1.0f;
+                factor[k] = there ? scales.x * a.scale_log2 : 0.0f, offset[k] = log2_fast(scale), inverse[k] = reciprocal_fast(scale);
+            }
+            if (!(token >= all_low && token + STEP <= min(all_high, end))) {
+                // what is hidden: its score becomes -infinity, and the block's factor, if it is 0, something that leaves it that
+#pragma unroll
+                for (int k = 0; k < BLOCKS; ++k) {
+                    factor[k] = fmaxf(factor[k], LEAST_FACTOR);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = token + k * BLOCK + row8 + i / 2 * 8;
+                            if (at < row_low[n][i & 1] || at >= min(row_high[n][i & 1], end)) s[n][k][i] = -INFINITY;
+                        }
+                }
+            }
+            float weight[TILES][BLOCKS][4], l_next[TILES][2];
+            bool nothing = false;  // a row that has seen nothing yet
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) nothing |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+            bool again = __any_sync(0xffffffffu, nothing);
+            while (true) {
+                if (again) {
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float top = m[n][i];
+#pragma unroll
+                            for (int k = 0; k < BLOCKS; ++k) top = fmaxf(top, fmaf(fmaxf(s[n][k][i], s[n][k][2 + i]), factor[k], offset[k]));
+#pragma unroll
+                            for (int step = 4; step < 32; step *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+                            const float shrink = m[n][i] == -INFINITY ? 1.0f : exp2_fast(m[n][i] - top);
+                            m[n][i] = top, l[n][i] *= shrink;
+#pragma unroll
+                            for (int t = 0; t < DIM / 16; ++t) o[n][t][i] *= shrink, o[n][t][2 + i] *= shrink;
+                        }
+                }
+                float worst = 0.0f;
 #pragma unroll
                 for (int n = 0; n < TILES; ++n)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float top = m[n][i];
+                        const float base = (m[n][i] == -INFINITY ? 0.0f : m[n][i]) - P_SHIFT;
+                        l_next[n][i] = l[n][i];
 #pragma unroll
-                        for (int k = 0; k < BLOCKS; ++k) top = fmaxf(top, fmaf(fmaxf(s[n][k][i], s[n][k][2 + i]), factor[k], offset[k]));
+                        for (int k = 0; k < BLOCKS; ++k) {
+                            weight[n][k][i] = exp2_fast(fmaf(s[n][k][i], factor[k], offset[k] - base)), weight[n][k][2 + i] = exp2_fast(fmaf(s[n][k][2 + i], factor[k], offset[k] - base));
+                            const float sum = weight[n][k][i] + weight[n][k][2 + i];
+                            worst = fmaxf(worst, sum);
+                            l_next[n][i] = fmaf(sum, inverse[k], l_next[n][i]);
+                        }
+                    }
+                if (again || __all_sync(0xffffffffu, worst <= MOST_SUM)) break;
+                again = true;
+            }
+            uint32_t p[TILES][BLOCKS][2];
 #pragma unroll
-                        for (int step = 4; step < 32; step *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-                        const float shrink = m[n][i] == -INFINITY ? 1.0f : exp2_fast(m[n][i] - top);
-                        m[n][i] = top, l[n][i] *= shrink;
+            for (int n = 0; n < TILES; ++n) {
+                l[n][0] = l_next[n][0], l[n][1] = l_next[n][1];
 #pragma unroll
-                        for (int t = 0; t < DIM / 16; ++t) o[n][t][i] *= shrink, o[n][t][2 + i] *= shrink;
+                for (int k = 0; k < BLOCKS; ++k)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const __half2 pair = __floats2half2_rn(weight[n][k][2 * r], weight[n][k][2 * r + 1]);
+                        p[n][k][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&pair));
                     }
             }
-            float worst = 0.0f;
 #pragma unroll
-            for (int n = 0; n < TILES; ++n)
+            for (int k = 0; k < BLOCKS; ++k) {
+                uint32_t value[4][V_WORDS];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float base = (m[n][i] == -INFINITY ? 0.0f : m[n][i]) - P_SHIFT;
-                    l_next[n][i] = l[n][i];
-#pragma unroll
-                    for (int k = 0; k < BLOCKS; ++k) {
-                        weight[n][k][i] = exp2_fast(fmaf(s[n][k][i], factor[k], offset[k] - base)), weight[n][k][2 + i] = exp2_fast(fmaf(s[n][k][2 + i], factor[k], offset[k] - base));
-                        const float sum = weight[n][k][i] + weight[n][k][2 + i];
-                        worst = fmaxf(worst, sum);
-                        l_next[n][i] = fmaf(sum, inverse[k], l_next[n][i]);
+                for (int i = 0; i < 4; ++i) {
+                    const int t = quad * 2 + (i & 1) + 8 * (i >> 1);
+                    const uint8_t *at = stage + (STEP + k * BLOCK + t) * DIM + value_place<DIM>(t, row8 * DIM / 128) * 16;
+                    if constexpr (DIM == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(at);
+                        value[i][0] = w.x, value[i][1] = w.y, value[i][2] = w.z, value[i][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(at + row8 % 2 * 8);
+                        value[i][0] = w.x, value[i][1] = w.y;
                     }
                 }
-            if (again || __all_sync(0xffffffffu, worst <= MOST_SUM)) break;
-            again = true;
-        }
-        uint32_t p[TILES][BLOCKS][2];
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-            l[n][0] = l_next[n][0], l[n][1] = l_next[n][1];
+                for (int w = 0; w < V_WORDS; ++w) {
+                    // [channel 4w of two tokens, channel 4w + 1 of both], and 4w + 2, 4w + 3; tokens 8 further on likewise
+                    const uint32_t low0 = __byte_perm(value[0][w], value[1][w], 0x5140), high0 = __byte_perm(value[0][w], value[1][w], 0x7362);
+                    const uint32_t low8 = __byte_perm(value[2][w], value[3][w], 0x5140), high8 = __byte_perm(value[2][w], value[3][w], 0x7362);
+                    const uint32_t a0 = widen2<0x4140>(low0), a1 = widen2<0x4342>(low0), a2 = widen2<0x4140>(low8), a3 = widen2<0x4342>(low8);
+                    const uint32_t c0 = widen2<0x4140>(high0), c1 = widen2<0x4342>(high0), c2 = widen2<0x4140>(high8), c3 = widen2<0x4342>(high8);
 #pragma unroll
-            for (int k = 0; k < BLOCKS; ++k)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const __half2 pair = __floats2half2_rn(weight[n][k][2 * r], weight[n][k][2 * r + 1]);
-                    p[n][k][r] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&pair));
-                }
-        }
-#pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            uint32_t value[4][V_WORDS];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = quad * 2 + (i & 1) + 8 * (i >> 1);
-                const uint8_t *at = stage + (STEP + k * BLOCK + t) * DIM + value_place<DIM>(t, row8 * DIM / 128) * 16;
-                if constexpr (DIM == 128) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(at);
-                    value[i][0] = w.x, value[i][1] = w.y, value[i][2] = w.z, value[i][3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(at + row8 % 2 * 8);
-                    value[i][0] = w.x, value[i][1] = w.y;
+                    for (int n = 0; n < TILES; ++n) {
+                        mma_16x8x16(o[n][2 * w], a0, a1, a2, a3, p[n][k][0], p[n][k][1]);
+                        mma_16x8x16(o[n][2 * w + 1], c0, c1, c2, c3, p[n][k][0], p[n][k][1]);
+                    }
                 }
             }
+        }
+        __syncthreads();  // the unit before has been read from where warps are joined
+        // warps, then pieces
 #pragma unroll
-            for (int w = 0; w < V_WORDS; ++w) {
-                // [channel 4w of two tokens, channel 4w + 1 of both], and 4w + 2, 4w + 3; tokens 8 further on likewise
-                const uint32_t low0 = __byte_perm(value[0][w], value[1][w], 0x5140), high0 = __byte_perm(value[0][w], value[1][w], 0x7362);
-                const uint32_t low8 = __byte_perm(value[2][w], value[3][w], 0x5140), high8 = __byte_perm(value[2][w], value[3][w], 0x7362);
-                const uint32_t a0 = widen2<0x4140>(low0), a1 = widen2<0x4342>(low0), a2 = widen2<0x4140>(low8), a3 = widen2<0x4342>(low8);
-                const uint32_t c0 = widen2<0x4140>(high0), c1 = widen2<0x4342>(high0), c2 = widen2<0x4140>(high8), c3 = widen2<0x4342>(high8);
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-                    mma_16x8x16(o[n][2 * w], a0, a1, a2, a3, p[n][k][0], p[n][k][1]);
-                    mma_16x8x16(o[n][2 * w + 1], c0, c1, c2, c3, p[n][k][0], p[n][k][1]);
-                }
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int step = 4; step < 32; step *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], step);
+                const int row = n * 8 + quad * 2 + i;
+                if (row8 == 0) join_m[warp][row] = m[n][i], join_l[warp][row] = l[n][i];
+#pragma unroll
+                for (int t = 0; t < DIM / 16; ++t) *reinterpret_cast<float2 *>(&join_o[warp][row][row8 * (DIM / 8) + 2 * t]) = make_float2(o[n][t][i], o[n][t][2 + i]);
             }
+        __syncthreads();
+        const bool whole = first == 0 && last == span.rounds;
+        const long long unit = static_cast<long long>(b) * cache.heads + head;
+        // a CTA has at most two units that it shares: the one that goes on from the CTA before, and the one that goes on in the next
+        float *piece = a.partial + (2LL * blockIdx.x + (first == 0)) * PIECE;
+        const int owned = rows;
+        auto finish = [&](int row, int channel, float2 sum, float top, float total) {  // channels `channel`, `channel` + 1
+            const long long out_row = entry.first + row / a.group;
+            const int out_head = head * a.group + row % a.group;
+            const float factor = total > 0.0f ? __frcp_rn(total) : (total == 0.0f ? 0.0f : total);
+            *reinterpret_cast<__half2 *>(a.y + out_row * a.ld_y + out_head * DIM + channel) = __floats2half2_rn(sum.x * factor, sum.y * factor);
+            if (channel == 0 && a.lse != nullptr)
+                a.lse[out_row * a.heads + out_head] = total == 0.0f ? -INFINITY : 0.6931471805599453f * (top - P_SHIFT + log2f(total));
+        };
+        for (int item = threadIdx.x; item < owned * (DIM / 2); item += DECODE_THREADS) {
+            const int row = item / (DIM / 2), channel = item % (DIM / 2) * 2;
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < DECODE_WARPS; ++w) top = fmaxf(top, join_m[w][row]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < DECODE_WARPS; ++w) {
+                const float weight = exp2_fast(join_m[w][row] - base);
+                const float2 part = *reinterpret_cast<const float2 *>(&join_o[w][row][channel]);
+                total = fmaf(join_l[w][row], weight, total), sum.x = fmaf(part.x, weight, sum.x), sum.y = fmaf(part.y, weight, sum.y);
+            }
+            if (whole) {
+                finish(row, channel, sum, top, total);
+            } else {
+                *reinterpret_cast<float2 *>(piece + 2 * ROWS + row * DIM + channel) = sum;
+                if (channel == 0) piece[row] = top, piece[ROWS + row] = total;
+            }
+        }
+        if (!whole) {
+            const long long first_cta = cta_of(unit_round);
+            const int used = static_cast<int>(cta_of(unit_round + span.rounds - 1) - first_cta) + 1;
+            auto piece_at = [&](int i) { return a.partial + (2 * (first_cta + i) + (i == 0)) * PIECE; };
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) is_last = atomicAdd(a.arrivals + unit, 1) == used - 1;
+            __syncthreads();
+            if (is_last) {
+                __threadfence();
+                // Warps share the pieces, lanes the channels, four rows at a time (the last again where there are fewer: no branch stands between
+                // one load and the next, of which there have to be many under way; with a walk over rows one by one this took 17 us for 37 pieces).
+                constexpr int EACH = DIM / 32, AT_ONCE = 4;
+                for (int base = 0; base < owned; base += AT_ONCE) {
+                    float top[AT_ONCE], totals[AT_ONCE], sum[AT_ONCE][EACH];
+                    int rows_of[AT_ONCE];
+#pragma unroll
+                    for (int n = 0; n < AT_ONCE; ++n) {
+                        rows_of[n] = min(base + n, owned - 1);
+                        top[n] = -INFINITY, totals[n] = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < EACH; ++c) sum[n][c] = 0.0f;
+                    }
+                    for (int i = lane; i < used; i += 32)
+#pragma unroll
+                        for (int n = 0; n < AT_ONCE; ++n) top[n] = fmaxf(top[n], __ldcg(piece_at(i) + rows_of[n]));
+#pragma unroll
+                    for (int n = 0; n < AT_ONCE; ++n) {
+#pragma unroll
+                        for (int step = 16; step > 0; step /= 2) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], step));
+                    }
+#pragma unroll 4
+                    for (int i = warp; i < used; i += DECODE_WARPS) {
+                        const float *one = piece_at(i);
+#pragma unroll
+                        for (int n = 0; n < AT_ONCE; ++n) {
+                            const int row = rows_of[n];
+                            const float weight = exp2_fast(__ldcg(one + row) - (top[n] == -INFINITY ? 0.0f : top[n]));
+                            totals[n] = fmaf(__ldcg(one + ROWS + row), weight, totals[n]);
+                            float part[EACH];
+                            if constexpr (EACH == 4) {
+                                const float4 f = __ldcg(reinterpret_cast<const float4 *>(one + 2 * ROWS + row * DIM + lane * EACH));
+                                part[0] = f.x, part[1] = f.y, part[2] = f.z, part[3] = f.w;
+                            } else {
+                                const float2 f = __ldcg(reinterpret_cast<const float2 *>(one + 2 * ROWS + row * DIM + lane * EACH));
+                                part[0] = f.x, part[1] = f.y;
+                            }
+#pragma unroll
+                            for (int c = 0; c < EACH; ++c) sum[n][c] = fmaf(part[c], weight, sum[n][c]);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < AT_ONCE; ++n) {
+                        if (lane == 0) join_m[warp][rows_of[n]] = top[n], join_l[warp][rows_of[n]] = totals[n];
+#pragma unroll
+                        for (int c = 0; c < EACH; ++c) join_o[warp][rows_of[n]][lane * EACH + c] = sum[n][c];
+                    }
+                }
+                __syncthreads();
+                for (int item = threadIdx.x; item < owned * (DIM / 2); item += DECODE_THREADS) {
+                    const int row = item / (DIM / 2), channel = item % (DIM / 2) * 2;
+                    float all = 0.0f;
+                    float2 both = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < DECODE_WARPS; ++w) {
+                        const float2 part = *reinterpret_cast<const float2 *>(&join_o[w][row][channel]);
+                        all += join_l[w][row], both.x += part.x, both.y += part.y;
+                    }
+                    finish(row, channel, both, join_m[0][row], all);
+                }
+                if (threadIdx.x == 0) a.arrivals[unit] = 0;
+            }
+        }
+        // ---- the next unit ----
+        unit_round += span.rounds;
+        r = 0;
+        if (round < end_round && ++head == cache.heads) {
+            head = 0;
+            do span_of(++b, span);
+            while (span.rounds == 0 && b + 1 < batch.entries);
+            if (span.rounds == 0) break;  // lengths that changed while the kernel ran
         }
     }
     cp_async_wait<0>();
-    __syncthreads();  // the rings become the place where warps are joined
-
-    // warps, then pieces
-#pragma unroll
-    for (int n = 0; n < TILES; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int step = 4; step < 32; step *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], step);
-            const int row = n * 8 + quad * 2 + i;
-            if (row8 == 0) join_m[warp][row] = m[n][i], join_l[warp][row] = l[n][i];
-#pragma unroll
-            for (int t = 0; t < DIM / 16; ++t) *reinterpret_cast<float2 *>(&join_o[warp][row][row8 * (DIM / 8) + 2 * t]) = make_float2(o[n][t][i], o[n][t][2 + i]);
-        }
-    __syncthreads();
-    const long long unit = (static_cast<long long>(b) * cache.heads + head) * a.row_tiles + tile;
-    float *partial = a.partial + unit * a.splits * (ROWS * (DIM + 2));
-    const int owned = last_row - first_row + 1;
-    auto finish = [&](int row, int channel, float2 sum, float top, float total) {  // channels `channel`, `channel` + 1
-        const long long out_row = entry.first + (first_row + row) / a.group;
-        const int out_head = head * a.group + (first_row + row) % a.group;
-        const float factor = total > 0.0f ? __frcp_rn(total) : (total == 0.0f ? 0.0f : total);
-        *reinterpret_cast<__half2 *>(a.y + out_row * a.ld_y + out_head * DIM + channel) = __floats2half2_rn(sum.x * factor, sum.y * factor);
-        if (channel == 0 && a.lse != nullptr)
-            a.lse[out_row * a.heads + out_head] = total == 0.0f ? -INFINITY : 0.6931471805599453f * (top - P_SHIFT + log2f(total));
-    };
-    for (int item = threadIdx.x; item < owned * (DIM / 2); item += DECODE_THREADS) {
-        const int row = item / (DIM / 2), channel = item % (DIM / 2) * 2;
-        float top = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < DECODE_WARPS; ++w) top = fmaxf(top, join_m[w][row]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < DECODE_WARPS; ++w) {
-            const float weight = exp2_fast(join_m[w][row] - base);
-            const float2 part = *reinterpret_cast<const float2 *>(&join_o[w][row][channel]);
-            total = fmaf(join_l[w][row], weight, total), sum.x = fmaf(part.x, weight, sum.x), sum.y = fmaf(part.y, weight, sum.y);
-        }
-        if (used == 1) {
-            finish(row, channel, sum, top, total);
-        } else {
-            float *mine = partial + static_cast<long long>(split) * (ROWS * (DIM + 2));
-            *reinterpret_cast<float2 *>(mine + 2 * ROWS + row * DIM + channel) = sum;
-            if (channel == 0) mine[row] = top, mine[ROWS + row] = total;
-        }
-    }
-    if (used == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) is_last = atomicAdd(a.arrivals + unit, 1) == used - 1;
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-    // Warps share the pieces, lanes the channels, four rows at a time (the last again where there are fewer: no branch stands between
-    // one load and the next, of which there have to be many under way; with a walk over rows one by one this took 17 us for 37 pieces).
-    constexpr int PIECE = ROWS * (DIM + 2), EACH = DIM / 32, AT_ONCE = 4;
-    for (int first = 0; first < owned; first += AT_ONCE) {
-        float top[AT_ONCE], total[AT_ONCE], sum[AT_ONCE][EACH];
-        int rows_of[AT_ONCE];
-#pragma unroll
-        for (int r = 0; r < AT_ONCE; ++r) {
-            rows_of[r] = min(first + r, owned - 1);
-            top[r] = -INFINITY, total[r] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < EACH; ++c) sum[r][c] = 0.0f;
-        }
-        for (int i = lane; i < used; i += 32)
-#pragma unroll
-            for (int r = 0; r < AT_ONCE; ++r) top[r] = fmaxf(top[r], __ldcg(partial + static_cast<long long>(i) * PIECE + rows_of[r]));
-#pragma unroll
-        for (int r = 0; r < AT_ONCE; ++r) {
-#pragma unroll
-            for (int step = 16; step > 0; step /= 2) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], step));
-        }
-#pragma unroll 4
-        for (int i = warp; i < used; i += DECODE_WARPS) {
-            const float *one = partial + static_cast<long long>(i) * PIECE;
-#pragma unroll
-            for (int r = 0; r < AT_ONCE; ++r) {
-                const int row = rows_of[r];
-                const float weight = exp2_fast(__ldcg(one + row) - (top[r] == -INFINITY ? 0.0f : top[r]));
-                total[r] = fmaf(__ldcg(one + ROWS + row), weight, total[r]);
-                float part[EACH];
-                if constexpr (EACH == 4) {
-                    const float4 f = __ldcg(reinterpret_cast<const float4 *>(one + 2 * ROWS + row * DIM + lane * EACH));
-                    part[0] = f.x, part[1] = f.y, part[2] = f.z, part[3] = f.w;
-                } else {
-                    const float2 f = __ldcg(reinterpret_cast<const float2 *>(one + 2 * ROWS + row * DIM + lane * EACH));
-                    part[0] = f.x, part[1] = f.y;
-                }
-#pragma unroll
-                for (int c = 0; c < EACH; ++c) sum[r][c] = fmaf(part[c], weight, sum[r][c]);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < AT_ONCE; ++r) {
-            if (lane == 0) join_m[warp][rows_of[r]] = top[r], join_l[warp][rows_of[r]] = total[r];
-#pragma unroll
-            for (int c = 0; c < EACH; ++c) join_o[warp][rows_of[r]][lane * EACH + c] = sum[r][c];
-        }
-    }
-    __syncthreads();
-    for (int item = threadIdx.x; item < owned * (DIM / 2); item += DECODE_THREADS) {
-        const int row = item / (DIM / 2), channel = item % (DIM / 2) * 2;
-        float all = 0.0f;
-        float2 both = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < DECODE_WARPS; ++w) {
-            const float2 part = *reinterpret_cast<const float2 *>(&join_o[w][row][channel]);
-            all += join_l[w][row], both.x += part.x, both.y += part.y;
-        }
-        finish(row, channel, both, join_m[0][row], all);
-    }
-    if (threadIdx.x == 0) a.arrivals[unit] = 0;
 }
 
 }  // namespace kv
