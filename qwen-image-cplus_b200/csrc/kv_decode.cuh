@@ -86,6 +86,12 @@ __device__ __forceinline__ uint4 load_codes(const uint8_t *at) {  // read once b
     asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(at));
     return w;
 }
+// Quotients of what may need 64 bits but hardly ever does.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+    if (static_cast<unsigned long long>(a) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // The keys that row `row` of an entry (row = token * group + head of the group) sees: [low, high).
 __device__ __forceinline__ void visible(const Attention &a, const Entry &entry, int row, int &low, int &high) {
     const int position = entry.length - entry.count + row / a.group;
@@ -171,8 +177,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
     const long long wanted = max((total + LEAST_ROUNDS - 1) / LEAST_ROUNDS, units);
     const long long ctas = min(static_cast<long long>(gridDim.x), wanted);
     if (blockIdx.x >= ctas) return;
-    const long long first_round = blockIdx.x * total / ctas, end_round = (blockIdx.x + 1) * total / ctas;
-    auto cta_of = [&](long long round) { return ((round + 1) * ctas - 1) / total; };
+    const long long first_round = divide(blockIdx.x * total, ctas), end_round = divide((blockIdx.x + 1) * total, ctas);
+    auto cta_of = [&](long long round) { return divide((round + 1) * ctas - 1, total); };
     if (mine > 0 && before * cache.heads <= first_round && first_round < (before + mine) * cache.heads) {
         int b = from;
         for (span_of(b, found); (before + found.rounds) * cache.heads <= first_round && b + 1 < to; span_of(++b, found)) before += found.rounds;
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
     Span span;
     span_of(b, span);
     if (span.rounds == 0) return;
-    int head = static_cast<int>((first_round - unit_round) / span.rounds), r = static_cast<int>((first_round - unit_round) % span.rounds);
+    int head = static_cast<int>(divide(first_round - unit_round, span.rounds)), r = static_cast<int>(first_round - unit_round - static_cast<long long>(head) * span.rounds);
     unit_round += static_cast<long long>(head) * span.rounds;
 
     // Each warp has a ring of STAGES steps of its own in shared memory, filled by 16-byte asynchronous copies, 16 KB of them under way at
@@ -244,15 +250,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
         fetch(step);
         go_on();
     }
-    int step = 0;
-    for (long long round = first_round; round < end_round;) {
-        // ---- one unit ----
-        const Entry &entry = span.entry;
-        const int rows = entry.count * a.group, end = span.high;
-        const int first = r, last = static_cast<int>(min(static_cast<long long>(span.rounds), r + end_round - round));  // rounds of it that are this CTA's
-        uint32_t q[TILES][K_WORDS][2];
-        int row_low[TILES][2], row_high[TILES][2];  // of this lane's columns of S^T
-        int all_low, all_high, unused;              // what every row sees
+    uint32_t q[TILES][K_WORDS][2];
+    auto fetch_queries = [&](const Entry &entry, int head) {
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
             const int row = n * 8 + row8;
@@ -260,16 +259,28 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
 #pragma unroll
             for (int j = 0; j < DIM / 64; ++j) {
                 uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                if (row < rows) {
+                if (row < entry.count * a.group) {
                     const uint4 *at = reinterpret_cast<const uint4 *>(source + (quad + 4 * j) * 16);
                     w[0] = __ldg(at), w[1] = __ldg(at + 1);
                 }
                 q[n][4 * j][0] = w[0].x, q[n][4 * j][1] = w[0].y, q[n][4 * j + 1][0] = w[0].z, q[n][4 * j + 1][1] = w[0].w;
                 q[n][4 * j + 2][0] = w[1].x, q[n][4 * j + 2][1] = w[1].y, q[n][4 * j + 3][0] = w[1].z, q[n][4 * j + 3][1] = w[1].w;
             }
+        }
+    };
+    fetch_queries(span.entry, head);
+    int step = 0;
+    for (long long round = first_round; round < end_round;) {
+        // ---- one unit ----
+        const Entry entry = span.entry;
+        const int rows = entry.count * a.group, end = span.high;
+        const int first = r, last = static_cast<int>(min(static_cast<long long>(span.rounds), r + end_round - round));  // rounds of it that are this CTA's
+        int row_low[TILES][2], row_high[TILES][2];  // of this lane's columns of S^T
+        int all_low, all_high, unused;              // what every row sees
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) visible(a, entry, min(n * 8 + quad * 2 + i, rows - 1), row_low[n][i], row_high[n][i]);
-        }
         visible(a, entry, rows - 1, all_low, unused);
         visible(a, entry, 0, unused, all_high);
         float o[TILES][DIM / 16][4], m[TILES][2], l[TILES][2];
@@ -412,6 +423,22 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
             }
         }
         __syncthreads();  // the unit before has been read from where warps are joined
+        // the next unit's queries are asked for before this one's warps are joined
+        const bool whole = first == 0 && last == span.rounds;
+        const long long unit = static_cast<long long>(b) * cache.heads + head, unit_begin = unit_round, unit_end = unit_round + span.rounds;
+        const int unit_head = head;
+        unit_round = unit_end, r = 0;
+        bool more = round < end_round;
+        if (more && ++head == cache.heads) {
+            head = 0;
+            do {
+                ++b;
+                if (b == ahead_entry) span = ahead;  // which has been looked up already
+                else span_of(b, span);
+            } while (span.rounds == 0 && b + 1 < batch.entries);
+            more = span.rounds > 0;  // else lengths changed while the kernel ran
+        }
+        if (more) fetch_queries(span.entry, head);
         // warps, then pieces
 #pragma unroll
         for (int n = 0; n < TILES; ++n)
@@ -425,14 +452,12 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
                 for (int t = 0; t < DIM / 16; ++t) *reinterpret_cast<float2 *>(&join_o[warp][row][row8 * (DIM / 8) + 2 * t]) = make_float2(o[n][t][i], o[n][t][2 + i]);
             }
         __syncthreads();
-        const bool whole = first == 0 && last == span.rounds;
-        const long long unit = static_cast<long long>(b) * cache.heads + head;
         // a CTA has at most two units that it shares: the one that goes on from the CTA before, and the one that goes on in the next
         float *piece = a.partial + (2LL * blockIdx.x + (first == 0)) * PIECE;
         const int owned = rows;
         auto finish = [&](int row, int channel, float2 sum, float top, float total) {  // channels `channel`, `channel` + 1
             const long long out_row = entry.first + row / a.group;
-            const int out_head = head * a.group + row % a.group;
+            const int out_head = unit_head * a.group + row % a.group;
             const float factor = total > 0.0f ? __frcp_rn(total) : (total == 0.0f ? 0.0f : total);
             *reinterpret_cast<__half2 *>(a.y + out_row * a.ld_y + out_head * DIM + channel) = __floats2half2_rn(sum.x * factor, sum.y * factor);
             if (channel == 0 && a.lse != nullptr)
@@ -459,8 +484,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
             }
         }
         if (!whole) {
-            const long long first_cta = cta_of(unit_round);
-            const int used = static_cast<int>(cta_of(unit_round + span.rounds - 1) - first_cta) + 1;
+            const long long first_cta = cta_of(unit_begin);
+            const int used = static_cast<int>(cta_of(unit_end - 1) - first_cta) + 1;
             auto piece_at = [&](int i) { return a.partial + (2 * (first_cta + i) + (i == 0)) * PIECE; };
             __threadfence();
             __syncthreads();
@@ -531,15 +556,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
                 if (threadIdx.x == 0) a.arrivals[unit] = 0;
             }
         }
-        // ---- the next unit ----
-        unit_round += span.rounds;
-        r = 0;
-        if (round < end_round && ++head == cache.heads) {
-            head = 0;
-            do span_of(++b, span);
-            while (span.rounds == 0 && b + 1 < batch.entries);
-            if (span.rounds == 0) break;  // lengths that changed while the kernel ran
-        }
+        if (!more) break;
     }
     cp_async_wait<0>();
 }
