@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     const uint32_t tmem = *tmem_slot;
     grid_wait();
 
-    const int split = blockIdx.x, head = blockIdx.y / a.row_tiles, tile = blockIdx.y % a.row_tiles, b = blockIdx.z;
+    // the last rows first: under a causal mask they see the most tokens, and what is short fills up the end
+    const int split = blockIdx.x, head = blockIdx.y % cache.heads, tile = a.row_tiles - 1 - blockIdx.y / cache.heads, b = blockIdx.z;
     Entry entry;
     const bool sound = read_entry(batch, tables, cache.page_shift, b, a.max_length, entry);
     if (!sound && threadIdx.x == 0) complain(0xC040);
