@@ -628,3 +628,33 @@ def test_norm_of_rows_without_spread(qi):
     assert (y[:2] == 0).all()
     exact = norm_exact(x[2:].double(), qi.NORM_LAYER, 1e-6, qi)
     assert (y[2:].double() - exact).abs().max() <= 2.0 ** -10  # a mean of 1e4 in 32 bits is known to 2^-11 of a deviation
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------
+
+
+def test_the_example_runs_and_both_ways_agree(qi):
+    # Token by token, blocks of 16 tokens are rounded again as their scales grow: keys and values differ by a code or so, half a percent of a
+    # deviation, from those appended at once; an attention's result by about as much, and three blocks add that up to a few percent at
+    # most. Wrong pages, positions or masks give outputs that have nothing in common (1.4 apart).
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("cached_block", os.path.join(entry.ROOT, "examples", "cached_block.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    difference, stepwise = example.main()
+    assert difference <= 0.1
+    assert torch.isfinite(stepwise).all()
+
+
+def test_block_scales_of_shared_prompts_are_the_parents(qi):
+    # a fork reads the prompt that its parent appended: same attention, bit for bit, from shared pages and from the copied last one
+    store = Store(qi, 21, [75, 0, 0], page=32, spare=8, table_extra=2)
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda")
+    told = ints([9])
+    assert qi.kv_pages_fork_ex(store.cache, store.pages, ints([0, 0]), ints([1, 2]), 2, told, workspace) == 0
+    assert told.item() == 0
+    store.lengths_list = [75, 75, 75]
+    q = (torch.randn(1, 4, 128, device="cuda") * 1.5).half().expand(3, -1, -1).contiguous()
+    y = attend(qi, store, [0, 1, 2], [1, 1, 1], 4, q=q)
+    assert torch.equal(y[0], y[1]) and torch.equal(y[0], y[2])
