@@ -36,7 +36,7 @@ struct Prefill {
     static constexpr int OPERAND_BYTES = TILE_TOKENS * DIM * 2;        // of K, V, or half of Q
     static constexpr int Q_AT = 0, K_AT = 2 * OPERAND_BYTES, V_AT = 4 * OPERAND_BYTES, SCALES_AT = 6 * OPERAND_BYTES;
     static constexpr int PLACES_AT = SCALES_AT + SLOTS * TILE_BLOCKS * 16, BARRIERS_AT = PLACES_AT + SLOTS * TILE_BLOCKS * 8;
-    static constexpr int BARRIERS = 8 + 2 * SLOTS + 10 + 1;
+    static constexpr int BARRIERS = 8 + 3 * SLOTS + 10 + 1;
     static constexpr int SMEM_BYTES = BARRIERS_AT + BARRIERS * 8 + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     float4(*scales)[TILE_BLOCKS] = reinterpret_cast<float4(*)[TILE_BLOCKS]>(smem + P::SCALES_AT);  // factor, offset, 1 / sv of each block
     long long(*places)[TILE_BLOCKS] = reinterpret_cast<long long(*)[TILE_BLOCKS]>(smem + P::PLACES_AT);  // its token row
     uint64_t *barriers = reinterpret_cast<uint64_t *>(smem + P::BARRIERS_AT);
-    uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *slot_full = barriers + 8, *slot_empty = slot_full + SLOTS;
+    uint64_t *k_full = barriers, *k_empty = barriers + 2, *v_full = barriers + 4, *v_empty = barriers + 6, *place_full = barriers + 8, *slot_full = place_full + SLOTS, *slot_empty = slot_full + SLOTS;
     uint64_t *s_full = slot_empty + SLOTS, *p_full = s_full + 2, *o_done = s_full + 6, *q_full = s_full + 10;  // of p and o [half of a tile][half of the rows]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(barriers + P::BARRIERS);
     __shared__ int is_last;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             mbarrier_init(s_full + i, 1);
         }
         for (int i = 0; i < 4; ++i) mbarrier_init(p_full + i, 4), mbarrier_init(o_done + i, 1);
-        for (int i = 0; i < SLOTS; ++i) mbarrier_init(slot_full + i, 1), mbarrier_init(slot_empty + i, 1);
+        for (int i = 0; i < SLOTS; ++i) mbarrier_init(place_full + i, 1), mbarrier_init(slot_full + i, 1), mbarrier_init(slot_empty + i, 1);
         mbarrier_init(q_full, 8);
         fence_barrier_init();
     }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(second_at + to), "r"(widen2<0x4140>(w.z)), "r"(widen2<0x4342>(w.z)), "r"(widen2<0x4140>(w.w)), "r"(widen2<0x4342>(w.w)) : "memory");
                 }
             };
-            bool alive = tiles > 0 && mbarrier_wait_warp(slot_full, 0, &g_status, STATUS_WAIT_FULL | 0xC020, lane);
+            bool alive = tiles > 0 && mbarrier_wait_warp(place_full, 0, &g_status, STATUS_WAIT_FULL | 0xC020, lane);
             if (alive) fetch(0, 0), fetch(1, 0);
             for (int j = 0; j < tiles && alive; ++j) {
                 const int stage = j & 1, phase = j >> 1 & 1;
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     if (lane == 0) mbarrier_arrive(v_full + stage);
                     break;
                 }
-                if (!mbarrier_wait_warp(slot_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
+                if (!mbarrier_wait_warp(place_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
                 fetch(0, j + 1);
                 if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) { alive = false; break; }
                 widen(1, P::V_AT + stage * P::OPERAND_BYTES);
@@ -306,19 +306,16 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                 for (int j = 0; j < tiles; ++j) {
                     const int next_page = page_at(j + 1), token = begin + j * TILE_TOKENS + lane * BLOCK;
                     if (page < 0 || page >= cache.pages) complain(0xC041), page = 0;
-                    long long place = 0;
-                    float k_scale = 0.0f, v_scale = 1.0f;
-                    if (lane < TILE_BLOCKS && token < end) {
-                        place = token_row(cache, page, head, token);
-                        k_scale = __ldg(cache.scales[0] + place / BLOCK), v_scale = fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE);
-                    }
+                    const bool there = lane < TILE_BLOCKS && token < end;
+                    long long place = there ? token_row(cache, page, head, token) : 0;
+                    const float k_scale = there ? __ldg(cache.scales[0] + place / BLOCK) : 0.0f, v_scale = there ? fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE) : 1.0f;
                     const long long first_place = __shfl_sync(0xffffffffu, place, 0);  // there is a token in the tile's first block
-                    if (token >= end) place = first_place;                             // what is fetched for nothing is masked, and finite
+                    if (!there) place = first_place;                                   // what is fetched for nothing is masked, and finite
                     if (j >= SLOTS && !mbarrier_wait_warp(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, &g_status, STATUS_WAIT_EMPTY | 0xC240, lane)) break;
-                    if (lane < TILE_BLOCKS) {
-                        places[j % SLOTS][lane] = place;
-                        scales[j % SLOTS][lane] = make_float4(fmaxf(k_scale * a.scale_log2, LEAST_FACTOR), log2_fast(v_scale), reciprocal_fast(v_scale), 0.0f);
-                    }
+                    if (lane < TILE_BLOCKS) places[j % SLOTS][lane] = place;
+                    __syncwarp();
+                    if (lane == 0) mbarrier_arrive(place_full + j % SLOTS);  // codes can be fetched while the scales are on their way
+                    if (lane < TILE_BLOCKS) scales[j % SLOTS][lane] = make_float4(fmaxf(k_scale * a.scale_log2, LEAST_FACTOR), log2_fast(v_scale), reciprocal_fast(v_scale), 0.0f);
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(slot_full + j % SLOTS);
                     page = next_page;
@@ -332,15 +329,31 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             const uint32_t s_at = tmem + lanes + TMEM_S + part * 128, o_at = tmem + lanes + TMEM_O + part * 128;
             int row_low, row_high;
             visible(a, entry, min(row, last_row), row_low, row_high);
+            // rows of Q and y in whole lines: a lane has piece `piece` of rows row0, row0 + ROWS_AT_ONCE, ... of its warp's 32
+            constexpr int PIECES = DIM / 8, ROWS_AT_ONCE = 32 / PIECES, WARP_PASSES = 32 / ROWS_AT_ONCE;
+            const int piece = lane % PIECES, y_row0 = first_row + part * TILE_ROWS + (warp & 3) * 32 + lane / PIECES, row0 = min(y_row0, rows - 1);
+            struct Walk {  // token and head of the group of a row, without a division a row
+                int token, member, tokens, members, group;
+                __device__ Walk(int row, int group) : token(row / group), member(row % group), tokens(ROWS_AT_ONCE / group), members(ROWS_AT_ONCE % group), group(group) {}
+                __device__ void go_on() {
+                    token += tokens, member += members;
+                    if (member >= group) member -= group, ++token;
+                }
+            };
             {
-                // this thread's row of Q
-                const __half *source = a.q + (entry.first + static_cast<long long>(row / a.group)) * a.ld_q + (head * a.group + row % a.group) * DIM;
-                const uint32_t r = (warp & 3) * 32 + lane, at = smem_u32(smem + P::Q_AT) + part * P::OPERAND_BYTES + r * 128;
+                // this warp's rows of Q, whole lines at a time: with a row to a thread the loads alone took 2 us
+                const uint32_t at = smem_u32(smem + P::Q_AT) + part * P::OPERAND_BYTES + piece / 8 * (TILE_ROWS * 128);
+                uint4 w[WARP_PASSES];
+                Walk walk(row0, a.group);
 #pragma unroll
-                for (int c = 0; c < DIM / 8; ++c) {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (row < rows) w = __ldg(reinterpret_cast<const uint4 *>(source) + c);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + c / 8 * (TILE_ROWS * 128) + ((c % 8 ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+                for (int i = 0; i < WARP_PASSES; ++i) {
+                    w[i] = __ldg(reinterpret_cast<const uint4 *>(a.q + (entry.first + static_cast<long long>(walk.token)) * a.ld_q + (head * a.group + walk.member) * DIM) + piece);
+                    if (row0 + (i + 1) * ROWS_AT_ONCE < rows) walk.go_on();  // beyond the last row: some row again, whose results are not written
+                }
+#pragma unroll
+                for (int i = 0; i < WARP_PASSES; ++i) {
+                    const uint32_t r = (warp & 3) * 32 + i * ROWS_AT_ONCE + lane / PIECES;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + r * 128 + ((piece % 8 ^ (r & 7)) << 4)), "r"(w[i].x), "r"(w[i].y), "r"(w[i].z), "r"(w[i].w) : "memory");
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -475,9 +488,9 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
 #pragma unroll
                             for (int c = 0; c < 32; ++c) o[c] = 0;
                         }
-                        if (row >= rows) continue;
                         if (used == 1) {
-                            uint4 *at = reinterpret_cast<uint4 *>(a.y + out_row * a.ld_y + out_head * DIM + i * 32);
+                            // through this warp's rows of Q, which is done with, so that rows leave in whole lines
+                            const uint32_t r = (warp & 3) * 32 + lane, at = smem_u32(smem + P::Q_AT) + part * P::OPERAND_BYTES + r * 128 + i / 2 * (TILE_ROWS * 128);
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t pairs[4];
@@ -486,12 +499,28 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                     const __half2 pair = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * e]) * factor, __uint_as_float(o[8 * c + 2 * e + 1]) * factor);
                                     pairs[e] = *reinterpret_cast<const uint32_t *>(&pair);
                                 }
-                                at[c] = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((i % 2 * 4 + c) ^ (r & 7)) << 4)), "r"(pairs[0]), "r"(pairs[1]), "r"(pairs[2]), "r"(pairs[3]) : "memory");
                             }
+                        } else if (row >= rows) {
+                            continue;
                         } else {
                             // a column's rows together: threads of a warp write adjacent words
 #pragma unroll
                             for (int c = 0; c < 32; ++c) partial[(2 + i * 32 + c) * PREFILL_ROWS + local] = __uint_as_float(o[c]);
+                        }
+                    }
+                    if (used == 1) {
+                        const uint32_t at = smem_u32(smem + P::Q_AT) + part * P::OPERAND_BYTES + piece / 8 * (TILE_ROWS * 128);
+                        Walk walk(row0, a.group);
+                        __syncwarp();
+#pragma unroll
+                        for (int n = 0; n < WARP_PASSES; ++n) {
+                            const uint32_t r = (warp & 3) * 32 + n * ROWS_AT_ONCE + lane / PIECES;
+                            uint4 w;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at + r * 128 + ((piece % 8 ^ (r & 7)) << 4)) : "memory");
+                            if (y_row0 + n * ROWS_AT_ONCE < rows)
+                                *(reinterpret_cast<uint4 *>(a.y + (entry.first + static_cast<long long>(walk.token)) * a.ld_y + (head * a.group + walk.member) * DIM) + piece) = w;
+                            walk.go_on();
                         }
                     }
                     if (row < rows && used == 1) {
