@@ -103,7 +103,9 @@ struct AttentionPlan {
     size_t partial_offset, bytes;
 };
 
-constexpr int DECODE_ROWS = 16;  // query rows to a sequence and head of the cache up to which a CTA of the streaming kernel holds all
+// Query rows to a sequence and head of the cache up to which the streaming kernel takes a call. 64 sequences of 2048 to 8192 tokens, 8 heads:
+// with 4 rows 123 us there and 324 on tcgen05, with 16 rows 152 and 393; one of 8192 with 16 rows 25 and 43. It has no form for more.
+constexpr int DECODE_ROWS = 16;
 
 // How a call is cut. The streaming kernel shares the tokens out by itself. The other one takes a CTA to a tile of rows, one to an SM, and
 // where there are too few tiles for the GPU, several to pieces of its tokens.
@@ -111,7 +113,9 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
     const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads), entries = batch->entries > 0 ? batch->entries : 1;
     plan.tiles = rows <= 8 ? 1 : rows <= DECODE_ROWS ? 2 : 0;
-    plan.grid = 2 * sms, plan.row_tiles = 1, plan.chunk = 0, plan.splits = 1;
+    plan.grid = sms * (cache->head_dim == 128 ? (plan.tiles == 1 ? kv::Decode<128, 1>::CTAS : kv::Decode<128, 2>::CTAS)
+                                              : (plan.tiles == 1 ? kv::Decode<64, 1>::CTAS : kv::Decode<64, 2>::CTAS));
+    plan.row_tiles = 1, plan.chunk = 0, plan.splits = 1;
     if (plan.tiles > 0) {
         plan.partial_offset = (static_cast<size_t>(entries) * cache->kv_heads * 4 + 255) / 256 * 256;
         // units of one round each are never shared

@@ -3,11 +3,13 @@
 //   y_i = sum_j softmax_j(scale * q_i . k_j) v_j       k_j = (c_j - 128) * sk, v_j = (d_j - 128) * sv, sk and sv one for 16 tokens
 //
 // The work is a list of rounds of 128 tokens: those of each unit (an entry and a head of the cache, with up to 8 * TILES query rows: group
-// heads times tokens) one after the other, unit after unit. Two CTAs an SM share it evenly, whatever the lengths, so that all end together
-// and each pays only once for its start; a ring of copies runs on from one unit into the next. A CTA's warps take 32 tokens of a round each,
+// heads times tokens) one after the other, unit after unit. Two or three CTAs an SM share it evenly, whatever the lengths, so that all
+// end together and each pays only once for its start; a ring of copies runs on from one unit into the next. A CTA's warps take 32 tokens of a round each,
 // with sums of their own; warps are joined in shared memory, and a unit that several CTAs share in a workspace, where the CTA that
-// arrives last adds the pieces up in their order (the same bits whichever is last). 64 sequences of 2048 to 8192 tokens, 8 heads, 131071
-// tokens of one: XX us, YY us; with a CTA to each piece of a unit 143 and 58.
+// arrives last adds the pieces up in their order (the same bits whichever is last). 64 sequences of
+// 2048 to 8192 tokens, 8 heads: 124 us, 5.1 TB/s (a CTA to each piece of a unit: 143); one of 131071: 62 us (58: pieces of one length
+// need no sharing out, but nobody knows beforehand). The slope with the length is 6.2 TB/s; what is left are 10 us of starting, joining
+// and launching. What bounds it: HBM, and the instructions that widen codes: 727 for 32 tokens and a warp, 45 % of the issue slots.
 //
 // The products run transposed on m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an instruction are tokens and channels
 // of the cache, of which there are always enough, and the 8 columns are queries, of which there may be one. Which channel or
@@ -20,8 +22,8 @@
 // cores; queries are float16 as they come, codes are exact, all sums are float32. m is not the maximum of what has been seen so far but an
 // older one: weights are computed with the m that there is, as 2^(x - m + 7), and only where one of them could be more than 2^15 is
 // the maximum taken anew and O rescaled. So float16 weights neither run over nor lose digits above 2^-21 of the largest, and what every
-// step would spend on a maximum over the warp (shuffles, one after the other) is spent in the first. A block of zeros has sv = 0: log2 is taken of max(sv, 2^-60), which changes
-// nothing that float16 results could hold.
+// step would spend on a maximum over the warp (shuffles, one after the other) is spent in the first. A block of zeros has sv = 0:
+// log2 is taken of max(sv, 2^-60), which changes nothing that float16 results could hold.
 #pragma once
 #include "kv_cache.cuh"
 
@@ -30,7 +32,7 @@ namespace kv {
 
 constexpr float P_SHIFT = 7.0f, MOST_SUM = 32768.0f, LEAST_SCALE = 8.6736174e-19f;  // 2^-60
 constexpr float LEAST_FACTOR = 1e-30f;  // in place of a key scale of zero: what is hidden stays -infinity times it, every score 0
-constexpr int DECODE_WARPS = 4, DECODE_THREADS = DECODE_WARPS * 32, STEP = 32, ROUND = DECODE_WARPS * STEP, LEAST_ROUNDS = 4;
+constexpr int DECODE_WARPS = 4, DECODE_THREADS = DECODE_WARPS * 32, STEP = 32, ROUND = DECODE_WARPS * STEP;
 
 struct Attention {
     const __half *q;
@@ -101,12 +103,16 @@ __device__ __forceinline__ void visible(const Attention &a, const Entry &entry, 
 
 template <int DIM, int TILES>
 struct Decode {
-    static constexpr int STAGES = DIM == 128 ? 3 : 5, STAGE_BYTES = 2 * STEP * DIM + 32;  // codes of keys, of values, scales
+    // CTAs to an SM, rounds of a ring, and rounds that are worth a CTA of their own (joining a piece costs as much). 64 sequences of 2048 to
+    // 8192 tokens, 8 heads: 128 channels, three CTAs with rings of two 124 us, two with three the same, but 131071 tokens of one 70 and 62;
+    // 64 channels 78 with three, 89 with two. With 16 rows two rounds, so that two CTAs fit: 163 us, 234 with one.
+    static constexpr int CTAS = DIM == 64 ? 3 : 2, LEAST_ROUNDS = TILES == 1 ? 2 : 4;
+    static constexpr int STAGES = (DIM == 64 ? 4 : 3) - (TILES == 1 ? 0 : 1), STAGE_BYTES = 2 * STEP * DIM + 32;  // codes of keys, of values, scales
     struct Join {
         float o[DECODE_WARPS][8 * TILES][DIM], m[DECODE_WARPS][8 * TILES], l[DECODE_WARPS][8 * TILES];
     };
     static constexpr int JOIN_AT = DECODE_WARPS * STAGES * STAGE_BYTES, SMEM_BYTES = JOIN_AT + sizeof(Join);
-    static_assert(TILES > 1 || 2 * (SMEM_BYTES + 1024 + 256) <= 228 * 1024, "two CTAs to an SM");
+    static_assert(CTAS * (SMEM_BYTES + 1024 + 128) <= 228 * 1024, "so many CTAs to an SM");
 };
 
 // Where piece `piece` (16 bytes) of a token's codes lies in its row: keys are read by lanes of two tokens in turn with four pieces each, values
@@ -117,7 +123,7 @@ template <int DIM>
 __device__ __forceinline__ int value_place(int token, int piece) { return DIM == 128 ? piece ^ (token >> 1 & 3) << 1 : piece ^ (token >> 1 & 3); }
 
 template <int DIM, int TILES>
-__global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, Tables tables, Batch batch, Attention a) {
+__global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) decode_kernel(Cache cache, Tables tables, Batch batch, Attention a) {
     constexpr int ROWS = 8 * TILES, K_WORDS = DIM / 16;            // K_WORDS: 32-bit words of a token's codes that a lane holds (keys)
     constexpr int V_WORDS = DIM / 32, BLOCKS = STEP / BLOCK;       // and of values, of each of four tokens
     constexpr int STAGES = Decode<DIM, TILES>::STAGES, STAGE_BYTES = Decode<DIM, TILES>::STAGE_BYTES;
@@ -174,6 +180,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 2) decode_kernel(Cache cache, 
     total *= cache.heads, units *= cache.heads;
     if (total == 0) return;
     // no more CTAs than have LEAST_ROUNDS each, or a unit: joining pieces costs as much as some rounds do
+    constexpr int LEAST_ROUNDS = Decode<DIM, TILES>::LEAST_ROUNDS;
     const long long wanted = max((total + LEAST_ROUNDS - 1) / LEAST_ROUNDS, units);
     const long long ctas = min(static_cast<long long>(gridDim.x), wanted);
     if (blockIdx.x >= ctas) return;
