@@ -195,6 +195,18 @@ def test_long_cache_is_split(qi):
     attend(qi, store, [0], [1], 8, max_length=64 * store.table.shape[1])
 
 
+@pytest.mark.parametrize("lengths", [[rng % 301 for rng in range(0, 4000, 97)], [5, 0, 131, 9000, 1, 0, 700], [0, 0, 40, 0], [3000] * 5])
+@pytest.mark.parametrize("entries", [2, 31, 129, 300])
+def test_batches_of_many_entries(qi, lengths, entries):
+    # more entries than threads, entries without queries or without tokens, short ones (a CTA to whole units) and long ones (units shared)
+    rng = random.Random(entries + len(lengths))
+    store = Store(qi, 9, lengths, kv_heads=1 if entries > 200 else 2)
+    slots = [rng.randrange(len(lengths)) for _ in range(entries)]
+    counts = [rng.choice((0, 1, 1, 1, 2)) for _ in slots]
+    counts[0] = 1
+    attend(qi, store, slots, counts, 4)
+
+
 def test_many_queries(qi):
     store = Store(qi, 4, [1500, 1300, 129], page=64, kv_heads=2)
     attend(qi, store, [0, 1, 2], [1500, 700, 129], 4)
