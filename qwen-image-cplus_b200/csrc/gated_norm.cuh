@@ -6,9 +6,10 @@
 // Each row is read once and written once; the values stay in registers between the sums, which are float32 and taken about the
 // mean (passes over registers, so that a large mean costs no digits). r' enters the second norm unrounded, also where it is
 // stored as float16. Bound by memory, and by what stands between a row's loads and its stores: up to four sums over the CTA. So each CTA
-// walks over its share of the rows with the next row's loads under way (three CTAs of 256 threads to an SM; 16384 rows of 4096: 156 us,
-// 5.2 TB/s; five CTAs without loads ahead 163, eight that do not all run at once 174). The vectors (gate, scale, shift, weights) come
-// from L1: a ring of rows in shared memory, filled by bulk copies, leaves no room for them there and took 203 us.
+// walks over its share of the rows with the next row's loads under way, and keeps what the vectors (gate, scale, shift, weights) come to
+// for a column in registers: two CTAs of 256 threads to an SM, 16384 rows of 4096: 132 us, 6.1 TB/s, 4096 rows 37.5. With the vectors
+// read from L1 for each row 156 (62 % of the issue slots were taken, most of them by that); five CTAs without loads ahead 163, eight that do
+// not all run at once 174; a ring of rows in shared memory, filled by bulk copies, leaves no L1 for the vectors: 203.
 #pragma once
 #include "ptx.cuh"
 
@@ -91,7 +92,7 @@ __device__ __forceinline__ float2 block_sums(float2 value, float2 (&sums)[2][WAR
 }
 
 template <int THREADS, int PIECES>
-__global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 768 / THREADS : 1) norm_kernel(const Arguments a) {
+__global__ void __launch_bounds__(THREADS, PIECES == 1 ? 768 / THREADS : THREADS == 256 ? 2 : 1) norm_kernel(const Arguments a) {
     constexpr int WARPS = THREADS / 32;
     __shared__ float2 sums[2][WARPS];
     grid_wait();
@@ -119,13 +120,17 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 768 / THREADS : 1) n
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum.x += x[p][j], sum.y = fmaf(x[p][j], x[p][j], sum.y);
+            for (int j = 0; j < 8; ++j) {
+                if (a.layer) sum.x += x[p][j];
+                sum.y = fmaf(x[p][j], x[p][j], sum.y);
+            }
         sum = block_sums<WARPS>(sum, sums, turn);
         if (!a.layer) return rsqrtf(fmaf(sum.y, per_value, a.epsilon));
         const float rest = sum.x * per_value;
         shift_by(rest);
         return rsqrtf(fmaxf(fmaf(sum.y, per_value, -rest * rest), 0.0f) + a.epsilon);
     };
+    constexpr bool KEEP = PIECES <= 2;  // a thread that has 32 columns has no registers for what follows, nor for a row ahead
     Raw8 raw_r[PIECES], raw_b[PIECES];  // the next row's values: on their way while this row's sums are waited for
     auto fetch = [&](long long row) {
 #pragma unroll
@@ -138,34 +143,67 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 768 / THREADS : 1) n
             }
         }
     };
-    fetch(blockIdx.x);
+    // What a column's values are multiplied by and what is added to them. They are kept for the rows to come, which mostly have the same vectors.
+    auto read_into = [&](int column, long long vector, float (&into)[8]) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) into[j] = a.residual_scale;
+        if (a.branch_weight != nullptr) {
+            load8(a.branch_weight, false, column, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) into[j] *= v[j];
+        }
+        if (a.gate != nullptr) {
+            load8(a.gate, a.vector_f16, vector + column, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) into[j] *= v[j];
+        }
+    };
+    auto read_out = [&](int column, long long vector, float (&scale)[8], float (&shift)[8]) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) scale[j] = 1.0f, shift[j] = 0.0f;
+        if (a.scale != nullptr) {
+            load8(a.scale, a.vector_f16, vector + column, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) scale[j] += v[j];
+        }
+        if (a.weight != nullptr) {
+            load8(a.weight, false, column, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) scale[j] *= v[j];
+        }
+        if (a.shift != nullptr) load8(a.shift, a.vector_f16, vector + column, shift);
+    };
+    constexpr int KEPT = KEEP ? PIECES : 1;
+    float into[KEPT][8], scale[KEPT][8], shift[KEPT][8];
+    if (KEEP) fetch(blockIdx.x);
+    long long held = -1;
     for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long start = static_cast<long long>(row) * a.width, vector = static_cast<long long>(row / a.rows_per_vector) * a.ld_vector;
+        if (KEEP && vector != held) {
+            held = vector;
+#pragma unroll
+            for (int p = 0; p < KEPT; ++p) {
+                const int column = (p * THREADS + threadIdx.x) * 8;
+                if (column < a.width) read_into(column, vector, into[p]), read_out(column, vector, scale[p], shift[p]);
+            }
+        }
+        if (!KEEP) fetch(row);
         float r[PIECES][8], b[PIECES][8];
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) widen8(raw_r[p], a.residual_f16, r[p]), widen8(raw_b[p], a.branch_f16, b[p]);
-        fetch(static_cast<long long>(row) + gridDim.x);
+        if (KEEP) fetch(static_cast<long long>(row) + gridDim.x);
         if (a.branch != nullptr) {
             const float factor = a.branch_norm ? normalise(b) : 1.0f;
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
                 const int column = (p * THREADS + threadIdx.x) * 8;
                 if (column >= a.width) continue;
-                float v[8];
+                float w[8];
+                if constexpr (!KEEP) read_into(column, vector, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) b[p][j] *= factor;
-                if (a.branch_weight != nullptr) {
-                    load8(a.branch_weight, false, column, v);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
-                }
-                if (a.gate != nullptr) {
-                    load8(a.gate, a.vector_f16, vector + column, v);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[p][j] *= v[j];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) r[p][j] = fmaf(a.residual_scale, b[p][j], r[p][j]);
+                for (int j = 0; j < 8; ++j) r[p][j] = fmaf(b[p][j] * factor, KEEP ? into[p % KEPT][j] : w[j], r[p][j]);
             }
         }
 #pragma unroll
@@ -179,24 +217,10 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 256 ? 768 / THREADS : 1) n
         for (int p = 0; p < PIECES; ++p) {
             const int column = (p * THREADS + threadIdx.x) * 8;
             if (column >= a.width) continue;
-            float v[8];
+            float w[8], v[8];
+            if constexpr (!KEEP) read_out(column, vector, w, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[p][j] *= factor;
-            if (a.weight != nullptr) {
-                load8(a.weight, false, column, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) r[p][j] *= v[j];
-            }
-            if (a.scale != nullptr) {
-                load8(a.scale, a.vector_f16, vector + column, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) r[p][j] *= 1.0f + v[j];
-            }
-            if (a.shift != nullptr) {
-                load8(a.shift, a.vector_f16, vector + column, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) r[p][j] += v[j];
-            }
+            for (int j = 0; j < 8; ++j) r[p][j] = fmaf(r[p][j] * factor, KEEP ? scale[p % KEPT][j] : w[j], KEEP ? shift[p % KEPT][j] : v[j]);
             store8(a.y, a.y_f16, start + column, r[p]);
         }
     }
