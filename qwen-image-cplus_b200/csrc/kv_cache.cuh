@@ -83,25 +83,30 @@ struct Unit {
     float *scale;
 };
 
-// False: nothing to do, or nothing that may be done.
-__device__ __forceinline__ bool read_unit(const Cache &cache, const Tables &tables, const Batch &batch, int dim, bool writes, uint32_t detail, Unit &u) {
-    const int lane = threadIdx.x & 31;
+// Which tokens of which block; false: nothing to do, or nothing that may be done.
+__device__ __forceinline__ bool read_unit(const Cache &cache, const Tables &tables, const Batch &batch, uint32_t detail, Unit &u) {
     const int unit = blockIdx.x * UNIT_WARPS + (threadIdx.x >> 5);  // (block, head, keys or values)
     u.which = unit & 1, u.head = (unit >> 1) % cache.heads;
     const bool sound = read_entry(batch, tables, cache.page_shift, blockIdx.y, 0x7fffffff, u.entry);
     if (!sound || u.entry.count > u.entry.length) {
-        if (lane == 0) complain(detail);
+        if ((threadIdx.x & 31) == 0) complain(detail);
         return false;
     }
     u.start = u.entry.length - u.entry.count, u.block = u.start / BLOCK + (unit >> 1) / cache.heads;
     const int first = u.block * BLOCK;
-    if (u.entry.count == 0 || first >= u.entry.length) return false;
+    u.early = max(u.start - first, 0), u.end = min(u.entry.length - first, BLOCK);
+    return u.entry.count > 0 && first < u.entry.length;
+}
+
+// Where the block is. The page's number and what it says about others are two trips to memory after the entry's two, so what does not depend
+// on them is asked for before.
+__device__ __forceinline__ bool place_unit(const Cache &cache, const Tables &tables, int dim, bool writes, uint32_t detail, Unit &u) {
+    const int first = u.block * BLOCK;
     const int page = __ldg(tables.table + static_cast<long long>(u.entry.slot) * tables.table_pages + (first >> cache.page_shift));
     if (page < 0 || page >= cache.pages || (writes && __ldg(tables.references + page) != 1)) {  // no page, or one that others hold too
-        if (lane == 0) complain(detail + 1);
+        if ((threadIdx.x & 31) == 0) complain(detail);
         return false;
     }
-    u.early = max(u.start - first, 0), u.end = min(u.entry.length - first, BLOCK);
     const long long row = token_row(cache, page, u.head, first);
     u.codes = (u.which == 0 ? cache.codes[0] : cache.codes[1]) + row * dim;
     u.scale = (u.which == 0 ? cache.scales[0] : cache.scales[1]) + row / BLOCK;
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) append_kernel(Cache cache, Ta
     grid_wait();
     const int lane = threadIdx.x & 31;
     Unit u;
-    if (!read_unit(cache, tables, batch, DIM, true, 0xC000, u)) return;
+    if (!read_unit(cache, tables, batch, 0xC000, u)) return;
     const int within = lane / LANES, channel = lane % LANES * CHANNELS;
     const T *source = (u.which == 0 ? k : v) + static_cast<long long>(u.head) * DIM + channel;
     const long long ld = u.which == 0 ? ld_k : ld_v, row0 = u.entry.first + static_cast<long long>(u.block) * BLOCK - u.start;
@@ -145,12 +150,13 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) append_kernel(Cache cache, Ta
         for (int j = 0; j < CHANNELS; ++j) x[i][j] = 0.0f;
         if (token >= u.early && token < u.end) load_values(source + (row0 + token) * ld, x[i]);
     }
+    if (!place_unit(cache, tables, DIM, true, 0xC001, u)) return;
+    const float old = u.early > 0 ? *u.scale : 0.0f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
 #pragma unroll
         for (int j = 0; j < CHANNELS; ++j) peak = fmaxf(peak, fabsf(x[i][j]));
     peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));  // no negative ones: ordered as whole numbers
-    const float old = u.early > 0 ? *u.scale : 0.0f;
     const float scale = fmaxf(old, __fmul_rn(peak, 1.0f / 127.0f));
     if (u.early > 0 && scale > old) {
         const float factor = __fdiv_rn(old, scale);
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) read_kernel(Cache cache, Tabl
     grid_wait();
     const int lane = threadIdx.x & 31;
     Unit u;
-    if (!read_unit(cache, tables, batch, DIM, false, 0xC010, u)) return;
+    if (!read_unit(cache, tables, batch, 0xC010, u) || !place_unit(cache, tables, DIM, false, 0xC011, u)) return;
     const int within = lane / LANES, channel = lane % LANES * 4;
     const float scale = *u.scale;
     uint32_t words[PASSES];
