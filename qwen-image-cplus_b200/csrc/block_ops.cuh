@@ -113,11 +113,13 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
     const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads), entries = batch->entries > 0 ? batch->entries : 1;
     plan.tiles = rows <= 8 ? 1 : rows <= DECODE_ROWS ? 2 : 0;
+    // One counter for each CTA of the streaming kernel or each tile of rows that is cut into pieces (at most half as many as SMs), at the same place
+    // for every call, so that calls of different shapes may share a workspace
+    plan.partial_offset = (static_cast<size_t>(sms) * 3 * 4 + 255) / 256 * 256;
     plan.grid = sms * (cache->head_dim == 128 ? (plan.tiles == 1 ? kv::Decode<128, 1>::CTAS : kv::Decode<128, 2>::CTAS)
                                               : (plan.tiles == 1 ? kv::Decode<64, 1>::CTAS : kv::Decode<64, 2>::CTAS));
     plan.row_tiles = 1, plan.chunk = 0, plan.splits = 1;
     if (plan.tiles > 0) {
-        plan.partial_offset = (static_cast<size_t>(entries) * cache->kv_heads * 4 + 255) / 256 * 256;
         // units of one round each are never shared
         plan.bytes = max_length <= kv::ROUND ? 0 : plan.partial_offset + static_cast<size_t>(plan.grid) * 2 * (8 * plan.tiles) * (cache->head_dim + 2) * 4;
         return true;
@@ -133,7 +135,6 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     chunk = (chunk + kv::TILE_TOKENS - 1) / kv::TILE_TOKENS * kv::TILE_TOKENS;
     if (chunk < kv::TILE_TOKENS) chunk = kv::TILE_TOKENS;
     plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(span > 0 ? (span + chunk - 1) / chunk : 1);
-    plan.partial_offset = (static_cast<size_t>(units) * 4 + 255) / 256 * 256;
     // room for as many pieces as any window gives
     const long long most = std::min(pieces, (max_length + kv::TILE_TOKENS - 1LL) / kv::TILE_TOKENS);
     plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * kv::PREFILL_ROWS * (cache->head_dim + 2) * 4 : 0;

@@ -44,7 +44,7 @@ struct Attention {
     float scale_log2;
     int causal, window, max_length;
     int chunk, splits, row_tiles;  // of the kernel for many queries
-    int *arrivals;      // one for each unit or tile of rows, zero between calls
+    int *arrivals;      // how many pieces are there, zero between calls: one for each CTA, for the unit that begins in it and goes on in the next, or for each tile of rows
     float *partial;     // what pieces leave: [piece][rows][head_dim + 2]
 };
 
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
         __syncthreads();  // the unit before has been read from where warps are joined
         // the next unit's queries are asked for before this one's warps are joined
         const bool whole = first == 0 && last == span.rounds;
-        const long long unit = static_cast<long long>(b) * cache.heads + head, unit_begin = unit_round, unit_end = unit_round + span.rounds;
+        const long long unit_begin = unit_round, unit_end = unit_round + span.rounds;
         const int unit_head = head;
         unit_round = unit_end, r = 0;
         bool more = round < end_round;
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
             auto piece_at = [&](int i) { return a.partial + (2 * (first_cta + i) + (i == 0)) * PIECE; };
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) is_last = atomicAdd(a.arrivals + unit, 1) == used - 1;
+            if (threadIdx.x == 0) is_last = atomicAdd(a.arrivals + first_cta, 1) == used - 1;
             __syncthreads();
             if (is_last) {
                 __threadfence();
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
                     }
                     finish(row, channel, both, join_m[0][row], all);
                 }
-                if (threadIdx.x == 0) a.arrivals[unit] = 0;
+                if (threadIdx.x == 0) a.arrivals[first_cta] = 0;
             }
         }
         if (!more) break;

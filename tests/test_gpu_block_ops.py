@@ -187,6 +187,22 @@ def test_rows_that_see_nothing(qi, heads):
     attend(qi, store, [0, 4], [1, 3], heads, causal=False)
 
 
+def test_calls_of_different_shapes_share_a_workspace(qi):
+    # counters of pieces lie where the partial results of another shape do not
+    store = Store(qi, 31, [9000, 700, 3000, 40, 2500, 1200] + [900] * 58, page=64)
+    dim, shapes = 128, [([0], [1], 2), (list(range(64)), [1] * 64, 16), ([2], [40], 2), (list(range(64)), [8] * 64, 2), ([0, 4], [33, 90], 6), (list(range(30)), [1] * 30, 2)]
+    batches = [store.batch(slots, counts) for slots, counts, _ in shapes]
+    workspace = torch.zeros(max(qi.kv_attention_workspace(store.cache, b, heads, 9000) for b, (_, _, heads) in zip(batches, shapes)), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        for batch, (slots, counts, heads) in zip(batches, shapes):
+            q = (torch.randn(sum(counts), heads, dim, device="cuda") * 1.5).half()
+            y = torch.full_like(q, float("nan"))
+            assert qi.kv_attention_ex(store.cache, store.pages, batch, store.layer, q, heads * dim, y, heads * dim, heads, dim ** -0.5, 9000, workspace=workspace) == 0
+            settled(qi)
+            exact, _ = attend_exact(store, q, slots, counts, heads, dim ** -0.5, True, 0)
+            assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm(), (counts, heads)
+
+
 def test_long_cache_is_split(qi):
     store = Store(qi, 3, [20011, 1, 9000], page=64)
     attend(qi, store, [0, 1, 2], [1, 1, 1], 8)
