@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_slot;
+    auto wait = [lane](uint64_t *barrier, uint32_t parity, uint32_t code) { return mbarrier_wait_warp(barrier, parity, &g_status, code, lane); };
     grid_wait();
 
     // the last rows first: under a causal mask they see the most tokens, and what is short fills up the end
@@ -224,26 +225,26 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(second_at + to), "r"(widen2<0x4140>(w.z)), "r"(widen2<0x4342>(w.z)), "r"(widen2<0x4140>(w.w)), "r"(widen2<0x4342>(w.w)) : "memory");
                 }
             };
-            bool alive = tiles > 0 && mbarrier_wait_warp(place_full, 0, &g_status, STATUS_WAIT_FULL | 0xC020, lane);
+            bool alive = tiles > 0 && wait(place_full, 0, STATUS_WAIT_FULL | 0xC020);
             if (alive) fetch(0, 0), fetch(1, 0);
             for (int j = 0; j < tiles && alive; ++j) {
                 const int stage = j & 1, phase = j >> 1 & 1;
-                if (!mbarrier_wait_warp(k_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC000 | stage, lane)) { alive = false; break; }
+                if (!wait(k_empty + stage, phase ^ 1, STATUS_WAIT_EMPTY | 0xC000 | stage)) { alive = false; break; }
                 widen(0, P::K_AT + stage * P::OPERAND_BYTES);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbarrier_arrive(k_full + stage);
                 if (j + 1 == tiles) {
-                    if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) break;
+                    if (!wait(v_empty + stage, phase ^ 1, STATUS_WAIT_EMPTY | 0xC100 | stage)) break;
                     widen(1, P::V_AT + stage * P::OPERAND_BYTES);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(v_full + stage);
                     break;
                 }
-                if (!mbarrier_wait_warp(place_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC020, lane)) { alive = false; break; }
+                if (!wait(place_full + (j + 1) % SLOTS, (j + 1) / SLOTS & 1, STATUS_WAIT_FULL | 0xC020)) { alive = false; break; }
                 fetch(0, j + 1);
-                if (!mbarrier_wait_warp(v_empty + stage, phase ^ 1, &g_status, STATUS_WAIT_EMPTY | 0xC100 | stage, lane)) { alive = false; break; }
+                if (!wait(v_empty + stage, phase ^ 1, STATUS_WAIT_EMPTY | 0xC100 | stage)) { alive = false; break; }
                 widen(1, P::V_AT + stage * P::OPERAND_BYTES);
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -253,56 +254,52 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
         } else if (warp >= ISSUE_WARP) {
             // ---- products ----
             setmaxnreg_dec<40>();
-            if (warp == ISSUE_WARP && tiles > 0) {
-                constexpr uint32_t IDESC_S = umma_idesc_f16_f32(TILE_ROWS, TILE_TOKENS), IDESC_O = umma_idesc_f16_f32(TILE_ROWS, DIM) | 1u << 16;  // B is MN-major
-                const uint32_t q_at = smem_u32(smem + P::Q_AT), k_at = smem_u32(smem + P::K_AT), v_at = smem_u32(smem + P::V_AT);
-                auto scores = [&](int i, int j) {
-                    const uint32_t q = q_at + i * P::OPERAND_BYTES, k = k_at + (j & 1) * P::OPERAND_BYTES;
+            if (warp == ISSUE_WARP) {
+                // One lane by itself: a vote of the warp or a hand-over to it at every step would be in the chain of the whole tile (471 us, so 464).
+                if (tiles > 0 && elect_one()) {
+                    constexpr uint32_t IDESC_S = umma_idesc_f16_f32(TILE_ROWS, TILE_TOKENS), IDESC_O = umma_idesc_f16_f32(TILE_ROWS, DIM) | 1u << 16;  // B is MN-major
+                    const uint32_t q_at = smem_u32(smem + P::Q_AT), k_at = smem_u32(smem + P::K_AT), v_at = smem_u32(smem + P::V_AT);
+                    auto scores = [&](int i, int j) {
+                        const uint32_t q = q_at + i * P::OPERAND_BYTES, k = k_at + (j & 1) * P::OPERAND_BYTES;
 #pragma unroll
-                    for (int s = 0; s < DIM / 16; ++s) {
-                        const uint32_t step = s / 4 * (TILE_TOKENS * 128) + s % 4 * 32;
-                        umma_f16(tmem + TMEM_S + i * 128, umma_desc_k_sw128(q + step), umma_desc_k_sw128(k + step), IDESC_S, s > 0);
+                        for (int s = 0; s < DIM / 16; ++s) {
+                            const uint32_t step = s / 4 * (TILE_TOKENS * 128) + s % 4 * 32;
+                            umma_f16(tmem + TMEM_S + i * 128, umma_desc_k_sw128(q + step), umma_desc_k_sw128(k + step), IDESC_S, s > 0);
+                        }
+                        tcgen05_commit(s_full + i);
+                    };
+                    bool alive = mbarrier_wait(q_full, 0, &g_status, STATUS_WAIT_FULL | 0xC200) && mbarrier_wait(k_full, 0, &g_status, STATUS_WAIT_FULL | 0xC210);
+                    tcgen05_fence_after();
+                    if (alive) {
+                        for (int i = 0; i < parts; ++i) scores(i, 0);
+                        tcgen05_commit(k_empty);
                     }
-                    tcgen05_commit(s_full + i);
-                };
-                bool alive = mbarrier_wait_warp(q_full, 0, &g_status, STATUS_WAIT_FULL | 0xC200, lane) && mbarrier_wait_warp(k_full, 0, &g_status, STATUS_WAIT_FULL | 0xC210, lane);
-                tcgen05_fence_after();
-                const bool elected = elect_one();
-                if (alive && elected) {
-                    for (int i = 0; i < parts; ++i) scores(i, 0);
-                    tcgen05_commit(k_empty);
-                }
-                __syncwarp();
-                for (int j = 0; j < tiles && alive; ++j) {
-                    const int stage = j & 1, next = (j + 1) & 1;
-                    alive = mbarrier_wait_warp(v_full + stage, j >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC220 | stage, lane);
-                    for (int i = 0; i < parts && alive; ++i) {
-                        for (int h = 0; h < 2; ++h) {
-                            alive = mbarrier_wait_warp(p_full + 2 * h + i, j & 1, &g_status, STATUS_WAIT_READY | 0xC230 | i, lane);
-                            if (!alive) break;
-                            tcgen05_fence_after();
-                            if (elected) {
+                    for (int j = 0; j < tiles && alive; ++j) {
+                        const int stage = j & 1, next = (j + 1) & 1;
+                        alive = mbarrier_wait(v_full + stage, j >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC220 | stage);
+                        for (int i = 0; i < parts && alive; ++i) {
+                            for (int h = 0; h < 2; ++h) {
+                                alive = mbarrier_wait(p_full + 2 * h + i, j & 1, &g_status, STATUS_WAIT_READY | 0xC230 | i);
+                                if (!alive) break;
+                                tcgen05_fence_after();
                                 const uint32_t v = v_at + stage * P::OPERAND_BYTES + h * (HALF_TOKENS * 128), weights = tmem + TMEM_S + i * 128 + h * 32;
 #pragma unroll
                                 for (int s = 0; s < HALF_TOKENS / 16; ++s)
                                     umma_f16_ts(tmem + TMEM_O + i * 128, weights + s * 8, umma_desc_mn_sw128(v + s * 2048, TILE_TOKENS * 128), IDESC_O, j + h > 0 || s > 0);
                                 tcgen05_commit(o_done + 2 * h + i);
                             }
-                            __syncwarp();
-                        }
-                        if (alive && i == 0 && j + 1 < tiles) alive = mbarrier_wait_warp(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next, lane);
-                        if (!alive) break;
-                        tcgen05_fence_after();
-                        if (elected) {
+                            if (alive && i == 0 && j + 1 < tiles) alive = mbarrier_wait(k_full + next, (j + 1) >> 1 & 1, &g_status, STATUS_WAIT_FULL | 0xC240 | next);
+                            if (!alive) break;
+                            tcgen05_fence_after();
                             if (j + 1 < tiles) scores(i, j + 1);
                             if (i == parts - 1) {
                                 tcgen05_commit(v_empty + stage), tcgen05_commit(slot_empty + j % SLOTS);
                                 if (j + 1 < tiles) tcgen05_commit(k_empty + next);
                             }
                         }
-                        __syncwarp();
                     }
                 }
+                __syncwarp();
             } else if (warp == LOOK_UP_WARP) {
                 const int *pages = tables.table + static_cast<long long>(entry.slot) * tables.table_pages;
                 auto page_at = [&](int j) {  // of this lane's block of tile j
@@ -318,7 +315,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     const float k_scale = there ? __ldg(cache.scales[0] + place / BLOCK) : 0.0f, v_scale = there ? fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE) : 1.0f;
                     const long long first_place = __shfl_sync(0xffffffffu, place, 0);  // there is a token in the tile's first block
                     if (!there) place = first_place;                                   // what is fetched for nothing is masked, and finite
-                    if (j >= SLOTS && !mbarrier_wait_warp(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, &g_status, STATUS_WAIT_EMPTY | 0xC240, lane)) break;
+                    if (j >= SLOTS && !wait(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, STATUS_WAIT_EMPTY | 0xC240)) break;
                     if (lane < TILE_BLOCKS) places[j % SLOTS][lane] = place;
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(place_full + j % SLOTS);  // codes can be fetched while the scales are on their way
@@ -370,8 +367,8 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
             bool alive = true;
             if (part < parts) {
                 for (int j = 0; j < tiles; ++j) {
-                    if (!mbarrier_wait_warp(slot_full + j % SLOTS, j / SLOTS & 1, &g_status, STATUS_WAIT_FULL | 0xC300 | part, lane) ||
-                        !mbarrier_wait_warp(s_full + part, j & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC300 | part, lane)) { alive = false; break; }
+                    if (!wait(slot_full + j % SLOTS, j / SLOTS & 1, STATUS_WAIT_FULL | 0xC300 | part) ||
+                        !wait(s_full + part, j & 1, STATUS_WAIT_TMEM_FULL | 0xC300 | part)) { alive = false; break; }
                     tcgen05_fence_after();
                     const int token = begin + j * TILE_TOKENS;
                     const int seen_low = row_low - token, seen_high = min(row_high, end) - token;
@@ -420,7 +417,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                                 const float shrink = m != -INFINITY ? exp2_fast(m - top) : 1.0f;
                                 m = top;
                                 if (j + h > 0) {
-                                    alive = mbarrier_wait_warp(o_done + 2 * (h ^ 1) + part, (h ? j : j - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC310 | part, lane);
+                                    alive = wait(o_done + 2 * (h ^ 1) + part, (h ? j : j - 1) & 1, STATUS_WAIT_TMEM_FULL | 0xC310 | part);
                                     if (!alive) break;
                                     tcgen05_fence_after();
 #pragma unroll 1
@@ -474,7 +471,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                     if (!alive) break;
                 }
                 if (alive && tiles > 0) {
-                    alive = mbarrier_wait_warp(o_done + 2 + part, (tiles - 1) & 1, &g_status, STATUS_WAIT_TMEM_FULL | 0xC320 | part, lane);
+                    alive = wait(o_done + 2 + part, (tiles - 1) & 1, STATUS_WAIT_TMEM_FULL | 0xC320 | part);
                     tcgen05_fence_after();
                 }
                 const long long unit = (static_cast<long long>(b) * cache.heads + head) * a.row_tiles + tile;
