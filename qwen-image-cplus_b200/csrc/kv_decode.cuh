@@ -7,9 +7,8 @@
 // end together and each pays only once for its start; a ring of copies runs on from one unit into the next. A CTA's warps take 32 tokens of a round each,
 // with sums of their own; warps are joined in shared memory, and a unit that several CTAs share in a workspace, where the CTA that
 // arrives last adds the pieces up in their order (the same bits whichever is last). 64 sequences of
-// 2048 to 8192 tokens, 8 heads: 124 us, 5.1 TB/s (a CTA to each piece of a unit: 143); one of 131071: 62 us (58: pieces of one length
-// need no sharing out, but nobody knows beforehand). The slope with the length is 6.2 TB/s; what is left are 10 us of starting, joining
-// and launching. What bounds it: HBM, and the instructions that widen codes: 727 for 32 tokens and a warp, 45 % of the issue slots.
+// 2048 to 8192 tokens, 8 heads: 120 us, 5.3 TB/s (a CTA to each piece of a unit: 143); one of 131071: 57 us. The slope with the length is 6.2 TB/s; what is left are 10 us of starting, joining
+// and launching. What bounds it: HBM, and the instructions that widen codes: 733 for 32 tokens and a warp, 48 % of the issue slots.
 //
 // The products run transposed on m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the 16 rows of an instruction are tokens and channels
 // of the cache, of which there are always enough, and the 8 columns are queries, of which there may be one. Which channel or

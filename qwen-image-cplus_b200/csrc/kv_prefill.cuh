@@ -18,12 +18,13 @@
 // maximum taken, O rescaled (which waits for the product before) and the pass repeated. So no weight is more than 2^15 in float16, and
 // all its digits are kept down to 2^-21 of the largest; sums are float32. Only the first tile pays for a pass over its maximum.
 //
-// Two guided sequences of 4096 and about 1600 queries over 4173 tokens, 32 heads: 470 us, 877 TFLOP/s; 37 heads of 4096 by 4096 901 TFLOP/s. A
-// tile takes a CTA 2.33 us, of which the products alone would be 1.6 (two thirds of the tensor cores' rate: Q and K from shared memory are
+// Two guided sequences of 4096 and about 1600 queries over 4173 tokens, 32 heads: 463 us, 890 TFLOP/s; one round of CTAs over 65536 tokens 1030. A
+// tile takes a CTA 2.3 us, of which the products alone would be 1.6 (two thirds of the tensor cores' rate: Q and K from shared memory are
 // 128 bytes a clock, and the widened codes are written beside them); the rest is the chain scores - weights - product - next scores,
 // which two halves of rows overlap and do not fill (issue slots 38 %, special functions 40 %, tensor cores 42 % busy). A CTA starts for 5 us
 // and ends for 3. Tried without gain: scores in halves of 64 columns, so that no softmax waits (521 us: Q is read twice); an issuing warp for
-// each half (568); a quarter or half of the exponentials as polynomials (531, 564); the maximum taken first (493); predicated MMAs (550).
+// each half (568); a quarter or half of the exponentials as polynomials (531, 564); the maximum taken first (493); predicated MMAs (550);
+// serving whichever half is ready (641: asking two barriers in turn takes longer); waits with pauses, or by all lanes (470 to 500).
 //
 // TMEM: S and P of the halves at columns 0 and 128, O at 256 and 384.
 #pragma once
