@@ -334,9 +334,21 @@ int qi_gated_norm_ex(const qi_gated_norm *call, void *stream) {
     a.residual_f16 = call->residual_dtype == QI_DTYPE_F16, a.branch_f16 = call->branch_dtype == QI_DTYPE_F16;
     a.vector_f16 = call->vector_dtype == QI_DTYPE_F16, a.y_f16 = call->y_dtype == QI_DTYPE_F16;
     a.branch_norm = call->branch_norm != 0, a.layer = call->kind == QI_NORM_LAYER;
+    // Threads for whole widths: idle ones hold registers that a row in flight could have. 16384 rows of 512 columns with 64 threads 21 us, with 128
+    // 28; of 768 with 96 28, with 128 31; of 1280 with 160 46, with 256 58; of 1536 with 192 53, with 256 62. 8192 rows of 2560 with 160 48, with
+    // 256 56; of 3072 with 192 57, with 256 61. 4096 rows of 5120 with 320 55, with 512 65; of 6144 with 384 63, with 512 70. Of 224 or 448 no more
+    // fit than of 256 or 512, and nothing was gained.
+    if (a.width <= 512) return launch_norm<64, 1>(a, stream);
+    if (a.width <= 768) return launch_norm<96, 1>(a, stream);
     if (a.width <= 1024) return launch_norm<128, 1>(a, stream);
+    if (a.width <= 1280) return launch_norm<160, 1>(a, stream);
+    if (a.width <= 1536) return launch_norm<192, 1>(a, stream);
     if (a.width <= 2048) return launch_norm<256, 1>(a, stream);
+    if (a.width <= 2560) return launch_norm<160, 2>(a, stream);
+    if (a.width <= 3072) return launch_norm<192, 2>(a, stream);
     if (a.width <= 4096) return launch_norm<256, 2>(a, stream);
+    if (a.width <= 5120) return launch_norm<320, 2>(a, stream);
+    if (a.width <= 6144) return launch_norm<384, 2>(a, stream);
     if (a.width <= 8192) return launch_norm<512, 2>(a, stream);
     return launch_norm<512, 4>(a, stream);
 }

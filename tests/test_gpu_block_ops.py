@@ -585,7 +585,7 @@ def norm_exact(x, kind, epsilon, qi):
 
 
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-@pytest.mark.parametrize("rows,width", [(1, 8), (3, 64), (5, 1000), (2, 1024), (7, 2048), (300, 3080), (2, 4096), (9, 5120), (3, 8200), (2, 16384), (3000, 512)])
+@pytest.mark.parametrize("rows,width", [(1, 8), (3, 64), (5, 1000), (2, 1024), (7, 2048), (300, 3080), (2, 4096), (9, 5120), (3, 8200), (2, 16384), (3000, 512), (1700, 768), (4, 1016), (950, 1280), (5, 1288), (700, 1536), (500, 2504), (3, 2560), (350, 3072), (200, 6144)])
 def test_norms(qi, kind, rows, width):
     kind = qi.NORM_LAYER if kind == "layer" else qi.NORM_RMS
     g = torch.Generator(device="cuda").manual_seed(rows + width)
