@@ -204,7 +204,7 @@ int launch_copies(const qi_kv_cache *cache, const kv::PageTables &tables, const 
     pool.pages = cache->pages, pool.layers = cache->layers;
     pool.page_bytes = cache->kv_heads * cache->page_tokens * cache->head_dim;
     pool.page_scales = cache->kv_heads * (cache->page_tokens / kv::BLOCK);
-    return launch_grid(kv::copy_kernel, dim3(sms_or_usual() * 8), kv::COPY_THREADS, 0, stream, pool, count, static_cast<int>(fixed_count), sources, targets, tables, moved);
+    return launch_grid(kv::copy_kernel, dim3(sms_or_usual() * kv::COPY_CTAS), kv::COPY_THREADS, 0, stream, pool, count, static_cast<int>(fixed_count), sources, targets, tables, moved);
 }
 
 }  // namespace
