@@ -69,16 +69,18 @@ int launch_grid(void (*kernel)(Parameters...), dim3 grid, int threads, int smem_
     return static_cast<int>(launched(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...)));
 }
 
-// CTAs to an entry for the kernels that take a block of a head with each warp, of keys or of values; -1: too many.
-long long cache_grid(const qi_kv_cache *cache, const qi_kv_batch *batch) {
-    const long long blocks = (static_cast<long long>(batch->most) + 2 * kv::BLOCK - 2) / kv::BLOCK;  // that `most` tokens in a row can touch
+// CTAs to an entry for the kernels that take a block of a head with each warp, of keys or of values; -1: too many. `most` may be any bound, but no
+// sequence has more blocks than its row of the table, so a block's first token stays below 2 * MOST_TABLE_PAGES pages, far from 2^31.
+long long cache_grid(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch) {
+    const long long touched = (static_cast<long long>(batch->most) + 2 * kv::BLOCK - 2) / kv::BLOCK;  // by `most` tokens in a row
+    const long long blocks = std::min(touched, static_cast<long long>(pages->table_pages) * cache->page_tokens / kv::BLOCK);
     const long long grid = (blocks * cache->kv_heads * 2 + kv::UNIT_WARPS - 1) / kv::UNIT_WARPS;
     return grid > 0x7fffffff / kv::UNIT_WARPS ? -1 : grid;
 }
 
 template <typename T>
 int launch_append(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k, const void *v, long long ld_k, long long ld_v, void *stream) {
-    const long long grid = cache_grid(cache, batch);
+    const long long grid = cache_grid(cache, pages, batch);
     if (grid < 0) return INVALID;
     auto kernel = cache->head_dim == 128 ? kv::append_kernel<T, 128> : kv::append_kernel<T, 64>;
     return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::UNIT_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),
@@ -87,7 +89,7 @@ int launch_append(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
 
 template <typename T>
 int launch_read(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, void *k, void *v, long long ld_k, long long ld_v, void *stream) {
-    const long long grid = cache_grid(cache, batch);
+    const long long grid = cache_grid(cache, pages, batch);
     if (grid < 0) return INVALID;
     auto kernel = cache->head_dim == 128 ? kv::read_kernel<T, 128> : kv::read_kernel<T, 64>;
     return launch_grid(kernel, dim3(static_cast<unsigned>(grid), batch->entries), kv::UNIT_WARPS * 32, 0, stream, layer_of(cache, layer), tables_of(pages), batch_of(batch),

@@ -116,6 +116,19 @@ def test_unfit_arguments_of_the_cache(qi):
         assert call(c, p, ctypes.byref(batch(qi, most=0, tokens=0)), 0, 256, 512, qi.DTYPE_F32, 512, 512, None) == 0
 
 
+@pytest.mark.parametrize("kv_heads", [1, 4, 64, 4096])
+def test_any_bound_of_new_tokens_is_cut_to_what_a_table_holds(qi, kv_heads):
+    # 5 pages of 32 tokens: 10 blocks a head, whatever `most` says; units of blocks that no sequence can have overflowed their token numbers
+    torch = pytest.importorskip("torch")
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    library, c, p, width = qi.lib(), cache(qi, kv_heads=kv_heads), pages(qi), kv_heads * 128
+    for most in (160, 161, 1 << 20, 0x7fffffff - 30, 0x7fffffff):
+        b = batch(qi, most=most)
+        for call in (library.qi_kv_append_ex, library.qi_kv_read_ex):
+            assert without_a_device(call(ctypes.byref(c), ctypes.byref(p), ctypes.byref(b), 1, 256, 512, qi.DTYPE_F16, width, width, None))
+
+
 @pytest.mark.parametrize("changes", [dict(layer=2), dict(layer=-1), dict(heads=0), dict(heads=6), dict(heads=-4), dict(heads=4 << 20), dict(q=0), dict(q=264), dict(y=0), dict(y=8), dict(lse=2), dict(ld_q=1016),
                                      dict(ld_y=1020), dict(ld_q=1028), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1),
                                      dict(max_length=-1)], ids=str)

@@ -380,6 +380,24 @@ def test_append_of_zeros_and_of_extremes(qi):
     assert (y == 0).all()
 
 
+@pytest.mark.parametrize("kv_heads", [1, 4, 9])
+def test_append_and_read_without_a_bound_of_new_tokens(qi, kv_heads):
+    lengths, counts = [333, 5, 40], [300, 1, 40]
+    a, b = (Store(qi, 19, lengths, kv_heads=kv_heads, table_extra=2) for _ in range(2))
+    rows, kv = make_kv(a, sum(counts), torch.float16, 20)
+    width = a.kv_heads * a.head_dim
+    append_plain(b, kv, [0, 1, 2], counts)
+    batch = a.batch([0, 1, 2], counts, most=0x7fffffff)
+    assert qi.kv_append_ex(a.cache, a.pages, batch, 1, rows, rows[:, width:], qi.DTYPE_F16, 2 * width, 2 * width) == 0
+    out = torch.full((2, sum(counts), width), float("nan"), device="cuda")
+    assert qi.kv_read_ex(a.cache, a.pages, batch, 1, out[0], out[1], qi.DTYPE_F32, width, width) == 0
+    settled(qi)
+    assert same_bytes(a, b)
+    for i, which in enumerate("kv"):
+        expected = torch.cat([a.values(which, s)[-n:] for s, n in zip((0, 1, 2), counts)]).float()
+        assert torch.equal(out[i].view(expected.shape), expected)
+
+
 def test_append_leaves_shared_and_missing_pages_alone(qi):
     # page numbers are the device's own: what must not be written is left as it is, and the status word says so
     for fault in ("shared", "missing", "foreign", "count", "slot"):
