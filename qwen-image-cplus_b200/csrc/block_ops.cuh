@@ -109,6 +109,9 @@ struct AttentionPlan {
 // with 4 rows 123 us there and 324 on tcgen05, with 16 rows 152 and 393; one of 8192 with 16 rows 25 and 43. It has no form for more.
 constexpr int DECODE_ROWS = 16;
 
+// A bound of lengths, cut to the tokens of a row of the table: at most 2^27, so that no piece of it leaves int and a loose bound costs nothing.
+int held_length(const qi_kv_cache *cache, int table_pages, int max_length) { return std::min(max_length, table_pages * cache->page_tokens); }
+
 // How a call is cut. The streaming kernel shares the tokens out by itself. The other one takes a CTA to a tile of rows, one to an SM, and
 // where there are too few tiles for the GPU, several to pieces of its tokens.
 bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int window, int sms, AttentionPlan &plan) {
@@ -235,7 +238,7 @@ int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
 
 int qi_kv_attention_workspace(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, size_t *bytes) {
     AttentionPlan plan;
-    if (!sound(cache) || !sound(batch) || !bytes || !plan_attention(cache, batch, heads, max_length, 0, sms_or_usual(), plan)) return INVALID;
+    if (!sound(cache) || !sound(batch) || !bytes || !plan_attention(cache, batch, heads, held_length(cache, kv::MOST_TABLE_PAGES, max_length), 0, sms_or_usual(), plan)) return INVALID;
     *bytes = plan.bytes;
     return 0;
 }
@@ -247,8 +250,9 @@ int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const
     if (!call->q || !call->y || !aligned16(call->q) || !aligned16(call->y) || !aligned4(call->lse) || call->ld_q < width || call->ld_y < width || call->ld_q % 8 != 0 ||
         call->ld_y % 8 != 0 || !(call->scale > 0.0f) || !(call->scale < INFINITY))
         return INVALID;
+    const int max_length = held_length(cache, pages->table_pages, call->max_length);
     AttentionPlan plan;
-    if (!plan_attention(cache, batch, call->heads, call->max_length, call->window, sms_or_usual(), plan)) return INVALID;
+    if (!plan_attention(cache, batch, call->heads, max_length, call->window, sms_or_usual(), plan)) return INVALID;
     if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes)) return INVALID;
     if (batch->entries == 0 || batch->most == 0) return 0;
     kv::Attention a;
@@ -256,7 +260,7 @@ int qi_kv_attention_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const
     a.ld_q = call->ld_q, a.ld_y = call->ld_y;
     a.heads = call->heads, a.group = call->heads / cache->kv_heads;
     a.scale_log2 = call->scale * 1.4426950408889634f;
-    a.causal = call->causal, a.window = call->window, a.max_length = call->max_length;
+    a.causal = call->causal, a.window = call->window, a.max_length = max_length;
     a.chunk = plan.chunk, a.splits = plan.splits, a.row_tiles = plan.row_tiles;
     a.arrivals = static_cast<int *>(workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.partial_offset);

@@ -211,6 +211,13 @@ def test_long_cache_is_split(qi):
     attend(qi, store, [0], [1], 8, max_length=64 * store.table.shape[1])
 
 
+@pytest.mark.parametrize("max_length", [0x7fffffff, 0x7fffffff - 127, 1 << 30, 1 << 27])
+@pytest.mark.parametrize("slots,counts", [(list(range(40)), [20 + s % 13 for s in range(40)]), ([3, 7], [25, 20]), (list(range(40)), [1] * 40)], ids=["one piece", "pieces", "streaming"])
+def test_any_bound_of_lengths(qi, max_length, slots, counts):
+    # 80 units of rows leave one piece of the tokens for each, which is then as long as the bound
+    attend(qi, Store(qi, 27, [50 + s for s in range(40)]), slots, counts, 2, max_length=max_length)
+
+
 @pytest.mark.parametrize("lengths", [[rng % 301 for rng in range(0, 4000, 97)], [5, 0, 131, 9000, 1, 0, 700], [0, 0, 40, 0], [3000] * 5])
 @pytest.mark.parametrize("entries", [2, 31, 129, 300])
 def test_batches_of_many_entries(qi, lengths, entries):
