@@ -97,7 +97,7 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
 // The keys that row `row` of an entry (row = token * group + head of the group) sees: [low, high).
 __device__ __forceinline__ void visible(const Attention &a, const Entry &entry, int row, int &low, int &high) {
     const int position = entry.length - entry.count + row / a.group;
-    low = a.window > 0 ? max(0, position - a.window + 1) : 0;
+    low = a.window > 0 && position >= a.window ? position - a.window + 1 : 0;  // (where there are more rows than tokens, positions go below zero)
     high = a.causal ? min(entry.length, position + 1) : entry.length;
 }
 

@@ -187,6 +187,14 @@ def test_rows_that_see_nothing(qi, heads):
     attend(qi, store, [0, 4], [1, 3], heads, causal=False)
 
 
+@pytest.mark.parametrize("window", [0x7fffffff, 0x7fffffff - 4, 1 << 30])
+@pytest.mark.parametrize("counts", [[5, 6], [30, 290]])
+@pytest.mark.parametrize("causal", [False, True])
+def test_any_window(qi, window, counts, causal):
+    # also for rows before the first token, whose positions are negative
+    attend(qi, Store(qi, 29, [3, 280]), [0, 1], counts, 2, causal=causal, window=window)
+
+
 def test_calls_of_different_shapes_share_a_workspace(qi):
     # counters of pieces lie where the partial results of another shape do not
     store = Store(qi, 31, [9000, 700, 3000, 40, 2500, 1200] + [900] * 58, page=64)
