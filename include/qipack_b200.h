@@ -483,7 +483,8 @@ int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
  * c tokens of a sequence of n stands at position p = n - c + i. `causal`: it sees tokens j <= p; `window` > 0: it sees
  * tokens j > p - window only. A row that sees nothing (no token, or p < 0) gives zeros. lse [tokens, heads] float32 or NULL
  * receives log sum_j exp(scale * q . k), -infinity for such a row, with which results over several caches can be
- * joined. Queries and weights enter the products as float16, codes exactly; all sums are float32. max_length bounds the
+ * joined. Queries and weights enter the products as float16, codes exactly; all sums are float32. Tokens whose
+ * page the table does not name soundly are hidden from all rows, an entry that is unsound leaves its rows of y and lse as they are, and the status word says so. max_length bounds the
  * lengths of the batch's sequences (0x7fffffff: whatever the table holds).
  * workspace: qi_kv_attention_workspace() bytes (0: none needed) for the same cache, batch bounds, heads and max_length, 16-byte
  * aligned, zeroed once before its first use; every call leaves its counters zero. Calls of any shapes that it is large enough for may share

@@ -237,18 +237,22 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
     Span ahead = span;
     int ahead_entry = b, ahead_head = head, ahead_round = r;
     long long left = end_round - first_round;
-    long long place[BLOCKS];  // token rows of its blocks; -1: none
+    long long place[BLOCKS];  // token rows of its blocks; -1: none, NO_PAGE: tokens whose page is no page of the pool, which nothing is read for
+    constexpr long long NO_PAGE = -2;
     auto look_up = [&]() {
         const int token = ahead.low + ahead_round * ROUND + warp * STEP;
         const int *pages = tables.table + static_cast<long long>(ahead.entry.slot) * tables.table_pages;
         auto place_of = [&](int token) -> long long {
             if (left <= 0 || token >= ahead.high) return -1;
-            int page = __ldg(pages + (token >> cache.page_shift));
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.pages)) complain(0xC031), page = 0;
+            const int page = __ldg(pages + (token >> cache.page_shift));
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.pages)) {
+                complain(0xC031);
+                return NO_PAGE;
+            }
             return token_row(cache, page, ahead_head, token);
         };
         place[0] = place_of(token);
-        if (cache.page_shift >= 5 && ahead.low % STEP == 0) place[1] = place[0] >= 0 && token + BLOCK < ahead.high ? place[0] + BLOCK : -1;  // in the same page
+        if (cache.page_shift >= 5 && ahead.low % STEP == 0) place[1] = token + BLOCK < ahead.high ? place[0] + (place[0] >= 0 ? BLOCK : 0) : -1;  // in the same page
         else place[1] = place_of(token + BLOCK);
     };
     static_assert(BLOCKS == 2, "look_up");
@@ -278,6 +282,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
                     cp_async_16(stage + (STEP + k * BLOCK + t) * DIM + value_place<DIM>(t, piece) * 16, cache.codes[1] + (place[k] + t) * DIM + piece * 16);
                 }
                 if (lane < 2) cp_async_4(stage + 2 * STEP * DIM + (2 * k + lane) * 4, (lane == 0 ? cache.scales[0] : cache.scales[1]) + place[k] / BLOCK);
+            } else if (place[k] == NO_PAGE && lane == 0) {
+                *reinterpret_cast<float2 *>(stage + 2 * STEP * DIM + 8 * k) = make_float2(0.0f, -1.0f);  // no scale is negative
             }
         }
         cp_async_commit();
@@ -359,9 +365,9 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
 #pragma unroll
             for (int k = 0; k < BLOCKS; ++k) {
                 const float2 scales = *reinterpret_cast<const float2 *>(stage + 2 * STEP * DIM + 8 * k);
-                const bool there = token + k * BLOCK < end;
-                const float scale = there ? fmaxf(scales.y, LEAST_SCALE) : 1.0f;
-                factor[k] = there ? scales.x * a.scale_log2 : 0.0f, offset[k] = log2_fast(scale), inverse[k] = reciprocal_fast(scale);
+                const bool there = token + k * BLOCK < end && !(scales.y < 0.0f);
+                const float scale = there ? fmaxf(scales.y, LEAST_SCALE) : 1.0f;  // else weights of 0, whatever the scores
+                factor[k] = there ? scales.x * a.scale_log2 : 0.0f, offset[k] = there ? log2_fast(scale) : -INFINITY, inverse[k] = reciprocal_fast(scale);
             }
             if (!(token >= all_low && token + STEP <= min(all_high, end))) {
                 // what is hidden: its score becomes -infinity, and the block's factor, if it is 0, something that leaves it that

@@ -310,17 +310,16 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
                 int page = page_at(0);
                 for (int j = 0; j < tiles; ++j) {
                     const int next_page = page_at(j + 1), token = begin + j * TILE_TOKENS + lane * BLOCK;
-                    if (page < 0 || page >= cache.pages) complain(0xC041), page = 0;
-                    const bool there = lane < TILE_BLOCKS && token < end;
-                    long long place = there ? token_row(cache, page, head, token) : 0;
+                    const bool known = page >= 0 && page < cache.pages, there = lane < TILE_BLOCKS && token < end && known;
+                    if (!known) complain(0xC041);
+                    // What is fetched for nothing (the pool's first codes) is finite, and its weights are 0: 2^-infinity, whatever the scores
+                    const long long place = there ? token_row(cache, page, head, token) : 0;
                     const float k_scale = there ? __ldg(cache.scales[0] + place / BLOCK) : 0.0f, v_scale = there ? fmaxf(__ldg(cache.scales[1] + place / BLOCK), LEAST_SCALE) : 1.0f;
-                    const long long first_place = __shfl_sync(0xffffffffu, place, 0);  // there is a token in the tile's first block
-                    if (!there) place = first_place;                                   // what is fetched for nothing is masked, and finite
                     if (j >= SLOTS && !wait(slot_empty + j % SLOTS, (j / SLOTS - 1) & 1, STATUS_WAIT_EMPTY | 0xC240)) break;
                     if (lane < TILE_BLOCKS) places[j % SLOTS][lane] = place;
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(place_full + j % SLOTS);  // codes can be fetched while the scales are on their way
-                    if (lane < TILE_BLOCKS) scales[j % SLOTS][lane] = make_float4(fmaxf(k_scale * a.scale_log2, LEAST_FACTOR), log2_fast(v_scale), reciprocal_fast(v_scale), 0.0f);
+                    if (lane < TILE_BLOCKS) scales[j % SLOTS][lane] = make_float4(fmaxf(k_scale * a.scale_log2, LEAST_FACTOR), there ? log2_fast(v_scale) : -INFINITY, reciprocal_fast(v_scale), 0.0f);
                     __syncwarp();
                     if (lane == 0) mbarrier_arrive(slot_full + j % SLOTS);
                     page = next_page;

@@ -288,6 +288,95 @@ def test_attention_in_a_graph_follows_lengths_on_the_device(qi, counts):
         assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm()
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [3, 8, 1, 2], [200, 30, 1, 150]])
+@pytest.mark.parametrize("fault", [-1, -(1 << 31), 0x7fffffff, "pages"])
+def test_attention_hides_tokens_without_a_page(qi, fault, counts, page, head_dim):
+    # what no sound page holds enters no result: neither page 0, which may be another sequence's, nor what lay in shared memory before
+    lengths, heads, group = [700, 330, 60, 150], 8, 4
+    store = Store(qi, 33, lengths, page=page, head_dim=head_dim)
+    for which in "kv":  # whatever is taken from elsewhere is large
+        store.codes[which][:] = store.codes[which].where(torch.rand(store.codes[which].shape, device="cuda") < 0.5, 255 - store.codes[which].clamp(1, 254))
+    held = [[which for which in range(-(-n // page))] for n in lengths]
+    gone = [[0], [1, len(held[1]) - 1], held[2], [2]]  # the first, a middle and the last, all of them
+    gone[0] += [j for j in held[0] if j % 3 == 2]
+    k, v = ([store.values(which, s) for s in range(4)] for which in "kv")
+    for s, missing in enumerate(gone):
+        for j in missing:
+            store.table[s, j] = len(store.references) if fault == "pages" else fault
+    tokens = sum(counts)
+    q = (torch.randn(tokens, heads, head_dim, device="cuda") * 1.5).half()
+    batch, y, lse = store.batch([0, 1, 2, 3], counts), torch.full_like(q, float("nan")), torch.full((tokens, heads), float("nan"), device="cuda")
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, batch, heads, 700), dtype=torch.uint8, device="cuda")
+    assert qi.kv_attention_ex(store.cache, store.pages, batch, 1, q, heads * head_dim, y, heads * head_dim, heads, head_dim ** -0.5, 700, lse=lse, workspace=workspace) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    begin = 0
+    for s, count in enumerate(counts):
+        p, j = torch.arange(lengths[s] - count, lengths[s], device="cuda")[:, None], torch.arange(lengths[s], device="cuda")[None]
+        hidden = (j > p) | torch.isin(j // page, torch.tensor(gone[s], device="cuda"))
+        mine = q[begin:begin + count].double()
+        scores = torch.einsum("ihd,jhd->hij", mine, k[s].repeat_interleave(group, 1)).mul(head_dim ** -0.5).masked_fill(hidden, -math.inf)
+        exact_lse = scores.logsumexp(2)
+        weights = torch.exp(scores - torch.where(exact_lse == -math.inf, 0.0, exact_lse)[..., None])
+        exact = torch.einsum("hij,jhd->ihd", weights, v[s].repeat_interleave(group, 1))
+        got, got_lse = y[begin:begin + count].double(), lse[begin:begin + count].T.double()
+        begin += count
+        seen = exact_lse > -math.inf
+        assert torch.equal(got_lse > -math.inf, seen) and not got.isnan().any() and (got.transpose(0, 1)[~seen] == 0).all()
+        assert (got - exact).abs().max() <= 2.0 ** -10 * v[s].abs().max() and (got - exact).norm() <= 2.0 ** -11 * exact.norm()
+        if seen.any():
+            assert (got_lse - exact_lse)[seen].abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [1, 200, 30]])
+@pytest.mark.parametrize("fault", ["slot", "negative slot", "length", "negative length", "offset"])
+def test_attention_and_read_leave_unsound_entries_alone(qi, fault, counts):
+    lengths, heads, dim = [400, 250, 300], 4, 128
+    store = Store(qi, 35, lengths, table_extra=8)
+    batch, tokens, bad = store.batch([0, 1, 2], counts), sum(counts), 1
+    q = (torch.randn(tokens, heads, dim, device="cuda") * 1.5).half()
+    exact, exact_lse = attend_exact(store, q, [0, 1, 2], counts, heads, dim ** -0.5, True, 0)
+    values = [torch.cat([store.values(which, s)[-n:] for s, n in zip((0, 1, 2), counts)]).float() for which in "kv"]
+    if fault == "slot":
+        batch.slots[1] = 3
+    elif fault == "negative slot":
+        batch.slots[1] = -1
+    elif fault == "length":
+        store.lengths[1] = 1 << 29  # more than a row of the table holds
+    elif fault == "negative length":
+        store.lengths[1] = -5
+    else:
+        batch.offsets[3], bad = tokens + 1, 2  # beyond the token rows
+    y, lse = torch.full_like(q, float("nan")), torch.full((tokens, heads), float("nan"), device="cuda")
+    out = torch.full((2, tokens, 2, dim), float("nan"), device="cuda")
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, batch, heads, 400), dtype=torch.uint8, device="cuda")
+    assert qi.kv_attention_ex(store.cache, store.pages, batch, 1, q, heads * dim, y, heads * dim, heads, dim ** -0.5, 400, lse=lse, workspace=workspace) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    assert qi.kv_read_ex(store.cache, store.pages, batch, 1, out[0], out[1], qi.DTYPE_F32, 2 * dim, 2 * dim) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    for s in range(3):
+        mine = slice(sum(counts[:s]), sum(counts[:s + 1]))
+        if s == bad:
+            assert y[mine].isnan().all() and lse[mine].isnan().all() and out[:, mine].isnan().all()
+        else:
+            assert (y[mine].double() - exact[mine]).norm() <= 2.0 ** -11 * exact[mine].norm() and (lse[mine].double() - exact_lse[mine]).abs().max() <= 1e-5
+            assert all(torch.equal(out[i, mine], values[i][mine]) for i in range(2))
+
+
+@pytest.mark.parametrize("fault", [-1, 0x7fffffff])
+def test_read_leaves_rows_without_a_page_alone(qi, fault):
+    store = Store(qi, 37, [100, 40], page=32)
+    values = [torch.cat([store.values(which, s) for s in (0, 1)]).float() for which in "kv"]
+    store.table[0, 1] = fault
+    out = torch.full((2, 140, 2, 128), float("nan"), device="cuda")
+    assert qi.kv_read_ex(store.cache, store.pages, store.batch([0, 1], [100, 40]), 1, out[0], out[1], qi.DTYPE_F32, 256, 256) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    assert out[:, 32:64].isnan().all()
+    for i in range(2):
+        assert torch.equal(out[i, :32], values[i][:32]) and torch.equal(out[i, 64:], values[i][64:])
+
+
 # ---- append and read back ------------------------------------------------------------------------------------------
 #
 # Codes and scales are equal to the definition's in 32 bits, bit for bit: products, divisions and roundings, each IEEE's.
