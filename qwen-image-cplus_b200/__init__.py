@@ -450,6 +450,40 @@ def _address(pointer):
     return pointer.data_ptr() if hasattr(pointer, "data_ptr") else pointer
 
 
+_dtype_names = {}
+_int32 = None  # torch's, once a tensor of it has been seen
+
+
+def _are(dtype: str, *tensors) -> bool:
+    """Whether all of them hold `dtype` and lie without gaps."""
+    global _int32
+    for t in tensors:
+        name = _dtype_names.get(t.dtype)
+        if name is None:
+            name = _dtype_names[t.dtype] = str(t.dtype).rpartition(".")[2]
+            if name == "int32":
+                _int32 = t.dtype
+        if name != dtype or not t.is_contiguous():
+            return False
+    return True
+
+
+def _reached(device, *tensors) -> bool:
+    """Whether a kernel on `device` can read and write all of them (which it also can in pinned host memory)."""
+    return all(t.device == device or t.is_pinned() for t in tensors)
+
+
+def _list(cache, values, count: int):
+    """The address of a list of `count` int32 beside `cache`; what is an address already is taken as it is."""
+    if not hasattr(values, "data_ptr"):
+        return values
+    if values.get_device() == cache.gpu and values.dtype is _int32 and values.numel() >= count and values.is_contiguous():
+        return values.data_ptr()  # these calls are short
+    if not _are("int32", values) or values.numel() < count or not _reached(cache.device, values):
+        raise ValueError(f"a list of {count} contiguous int32 on {cache.device} is wanted, not {values.numel()} of {values.dtype} on {values.device}")
+    return values.data_ptr()
+
+
 class KvCache:
     """The pool: codes uint8 [layers, pages, kv_heads, page_tokens, head_dim], scales float32 [layers, pages, kv_heads, page_tokens / 16]."""
 
@@ -458,8 +492,9 @@ class KvCache:
         layers, pages, kv_heads, page_tokens, head_dim = k_codes.shape
         if tuple(v_codes.shape) != tuple(k_codes.shape) or any(tuple(s.shape) != (layers, pages, kv_heads, page_tokens // KV_BLOCK) for s in (k_scales, v_scales)):
             raise ValueError("the codes and scales of a cache do not belong together")
-        if not all(t.is_contiguous() for t in (k_codes, v_codes, k_scales, v_scales)):
-            raise ValueError("the codes and scales of a cache are contiguous")
+        self.device, self.gpu = k_codes.device, k_codes.get_device() if k_codes.is_cuda else None
+        if not _are("uint8", k_codes, v_codes) or not _are("float32", k_scales, v_scales) or not _reached(self.device, v_codes, k_scales, v_scales):
+            raise ValueError("the codes of a cache are uint8, its scales float32, all contiguous and on one device")
         self.cache = qi_kv_cache(_p(k_codes), _p(v_codes), _p(k_scales), _p(v_scales), layers, pages, page_tokens, kv_heads, head_dim)
         self.reference = ctypes.byref(self.cache)
 
@@ -470,10 +505,19 @@ class KvPages:
     def __init__(self, table, lengths, references):
         self.table, self.lengths, self.references = table, lengths, references
         sequences, table_pages = table.shape
-        if lengths.numel() != sequences or not all(t.is_contiguous() for t in (table, lengths, references)):
-            raise ValueError("a table of pages, its lengths and its references are contiguous and belong together")
+        if lengths.numel() != sequences or not _are("int32", table, lengths, references):
+            raise ValueError("a table of pages, its lengths and its references are contiguous int32 and belong together")
         self.pages = qi_kv_pages(_p(table), _p(lengths), _p(references), sequences, table_pages)
         self.reference = ctypes.byref(self.pages)
+        self.pool = None  # the one that it has been found to fit
+
+    def of(self, cache: KvCache):
+        """The C structure, for calls on `cache`."""
+        if self.pool is not cache:
+            if self.references.numel() < cache.cache.pages or not _reached(cache.device, self.table, self.lengths, self.references):
+                raise ValueError(f"{self.references.numel()} references on {self.references.device} for a pool of {cache.cache.pages} pages on {cache.device}")
+            self.pool = cache
+        return self.reference
 
 
 class KvBatch:
@@ -481,18 +525,31 @@ class KvBatch:
 
     def __init__(self, slots, offsets, tokens: int, most: int):
         self.slots, self.offsets = slots, offsets
-        self.batch = qi_kv_batch(_p(slots), _p(offsets), offsets.numel() - 1, tokens, most)
+        entries = offsets.numel() - 1
+        self.lists = (offsets,) if slots is None else (offsets, slots)
+        if entries < 0 or not _are("int32", *self.lists) or (slots is not None and slots.numel() < entries):
+            raise ValueError("a batch has contiguous int32: an offset more than entries, and a slot for each")
+        self.batch = qi_kv_batch(_p(slots), _p(offsets), entries, tokens, most)
         self.reference = ctypes.byref(self.batch)
+        self.pool = None  # the one that it has been found beside
+
+    def of(self, cache: KvCache):
+        """The C structure, for calls on `cache`."""
+        if self.pool is not cache:
+            if not _reached(cache.device, *self.lists):
+                raise ValueError(f"a batch on {self.offsets.device} for a pool on {cache.device}")
+            self.pool = cache
+        return self.reference
 
 
 def kv_append_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
     """Quantises the batch's keys and values into their pages."""
-    return lib().qi_kv_append_ex(cache.reference, pages.reference, batch.reference, layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
+    return lib().qi_kv_append_ex(cache.reference, pages.of(cache), batch.of(cache), layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
 
 
 def kv_read_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, k, v, dtype: int, ld_k: int, ld_v: int, stream=None) -> int:
     """The values that the cache holds for the batch's tokens."""
-    return lib().qi_kv_read_ex(cache.reference, pages.reference, batch.reference, layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
+    return lib().qi_kv_read_ex(cache.reference, pages.of(cache), batch.of(cache), layer, _address(k), _address(v), dtype, ld_k, ld_v, _address(stream))
 
 
 def _bytes_of(workspace) -> int:
@@ -512,13 +569,13 @@ def kv_attention_ex(cache: KvCache, pages: KvPages, batch: KvBatch, layer: int, 
                     causal: bool = True, window: int = 0, lse=None, workspace=None, stream=None) -> int:
     """y = attention of float16 q over the batch's sequences; lse float32 [tokens, heads] or None."""
     call = qi_kv_attention(layer, heads, _address(q), ld_q, _address(y), ld_y, _address(lse), scale, int(causal), window, max_length)
-    return lib().qi_kv_attention_ex(cache.reference, pages.reference, batch.reference, ctypes.byref(call), _address(workspace), _bytes_of(workspace), _address(stream))
+    return lib().qi_kv_attention_ex(cache.reference, pages.of(cache), batch.of(cache), ctypes.byref(call), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_workspace(cache: KvCache, pages: KvPages) -> int:
     """Bytes of workspace of the calls below."""
     value = ctypes.c_size_t(0)
-    status = lib().qi_kv_pages_workspace(cache.reference, pages.reference, ctypes.byref(value))
+    status = lib().qi_kv_pages_workspace(cache.reference, pages.of(cache), ctypes.byref(value))
     if status != 0:
         raise ValueError(f"no such cache (status {status})")
     return value.value
@@ -526,27 +583,27 @@ def kv_pages_workspace(cache: KvCache, pages: KvPages) -> int:
 
 def kv_pages_reserve_ex(cache: KvCache, pages: KvPages, slots, counts, count: int, shortage, workspace, stream=None) -> int:
     """Pages for counts[i] more tokens of sequence slots[i]; `shortage` (device int32): 0, or how many pages are missing."""
-    return lib().qi_kv_pages_reserve_ex(cache.reference, pages.reference, _address(slots), _address(counts), count, _address(shortage), _address(workspace), _bytes_of(workspace), _address(stream))
+    return lib().qi_kv_pages_reserve_ex(cache.reference, pages.of(cache), _list(cache, slots, count), _list(cache, counts, count), count, _list(cache, shortage, 1), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_fork_ex(cache: KvCache, pages: KvPages, parents, children, count: int, shortage, workspace, stream=None) -> int:
     """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call."""
-    return lib().qi_kv_pages_fork_ex(cache.reference, pages.reference, _address(parents), _address(children), count, _address(shortage), _address(workspace), _bytes_of(workspace), _address(stream))
+    return lib().qi_kv_pages_fork_ex(cache.reference, pages.of(cache), _list(cache, parents, count), _list(cache, children, count), count, _list(cache, shortage, 1), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_free_ex(cache: KvCache, pages: KvPages, slots, count: int, stream=None) -> int:
     """The sequences end and give their pages back."""
-    return lib().qi_kv_pages_free_ex(cache.reference, pages.reference, _address(slots), count, _address(stream))
+    return lib().qi_kv_pages_free_ex(cache.reference, pages.of(cache), _list(cache, slots, count), count, _address(stream))
 
 
 def kv_pages_compact_ex(cache: KvCache, pages: KvPages, used, workspace, stream=None) -> int:
     """Moves the pages in use together at the front; `used` (device int32) becomes their number."""
-    return lib().qi_kv_pages_compact_ex(cache.reference, pages.reference, _address(used), _address(workspace), _bytes_of(workspace), _address(stream))
+    return lib().qi_kv_pages_compact_ex(cache.reference, pages.of(cache), _list(cache, used, 1), _address(workspace), _bytes_of(workspace), _address(stream))
 
 
 def kv_pages_copy_ex(cache: KvCache, sources, targets, count: int, stream=None) -> int:
     """Copies page sources[i] to page targets[i] in every layer."""
-    return lib().qi_kv_pages_copy_ex(cache.reference, _address(sources), _address(targets), count, _address(stream))
+    return lib().qi_kv_pages_copy_ex(cache.reference, _list(cache, sources, count), _list(cache, targets, count), count, _address(stream))
 
 
 class GatedNorm:

@@ -194,3 +194,60 @@ def test_structures_that_do_not_belong_together(qi):
         qi.KvCache(codes, codes, scales, scales[..., :1])
     with pytest.raises(ValueError):
         qi.KvPages(torch.zeros(3, 5, dtype=torch.int32).T, torch.zeros(5, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+
+
+def test_structures_of_other_types_and_sizes(qi):
+    # what the device cannot see: int64 read as int32 pairs, scales of half the size written beyond, references shorter than the pool
+    torch = pytest.importorskip("torch")
+    codes, scales = torch.zeros(1, 4, 2, 32, 64, dtype=torch.uint8), torch.zeros(1, 4, 2, 2)
+    for k, v, ks, vs in ((codes.float(), codes, scales, scales), (codes.view(torch.int8), codes, scales, scales), (codes, codes.char(), scales, scales), (codes, codes, scales.half(), scales),
+                         (codes, codes, scales, scales.double()), (codes, codes, scales, scales.int()), (codes.to("meta"), codes, scales, scales), (codes, codes, scales, scales.to("meta"))):
+        with pytest.raises(ValueError):
+            qi.KvCache(k, v, ks, vs)
+    table, lengths, references = torch.zeros(3, 5, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    for parts in ((table.long(), lengths, references), (table, lengths.long(), references), (table, lengths, references.long()), (table.float(), lengths, references),
+                  (table, lengths, torch.zeros(8, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError):
+            qi.KvPages(*parts)
+    offsets, slots = torch.zeros(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for parts in ((slots, offsets.long()), (slots.long(), offsets), (slots[:2], offsets), (None, offsets[:0]), (None, offsets.float()), (torch.zeros(6, dtype=torch.int32)[::2], offsets)):
+        with pytest.raises(ValueError):
+            qi.KvBatch(*parts, 5, 2)
+    qi.KvBatch(None, offsets, 5, 2), qi.KvBatch(slots, offsets, 5, 2), qi.KvBatch(torch.zeros(9, dtype=torch.int32), offsets, 5, 2)
+
+
+def test_lists_and_pools_that_are_too_short(qi):
+    torch = pytest.importorskip("torch")
+    ints = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    cache_ = qi.KvCache(torch.zeros(1, 4, 2, 32, 64, dtype=torch.uint8), torch.zeros(1, 4, 2, 32, 64, dtype=torch.uint8), torch.zeros(1, 4, 2, 2), torch.zeros(1, 4, 2, 2))
+    pages_, batch_ = qi.KvPages(torch.zeros(3, 5, dtype=torch.int32), ints(3), ints(4)), qi.KvBatch(None, ints(3), 4, 2)
+    few = qi.KvPages(torch.zeros(3, 5, dtype=torch.int32), ints(3), ints(3))  # a reference less than pages
+    elsewhere = [qi.KvPages(*(t.to("meta") if i == part else t for i, t in enumerate((torch.zeros(3, 5, dtype=torch.int32), ints(3), ints(4))))) for part in range(3)]
+    work = torch.zeros(1 << 12, dtype=torch.uint8)
+    calls = [lambda p, l: qi.kv_pages_reserve_ex(cache_, p, l, ints(3), 3, ints(1), work), lambda p, l: qi.kv_pages_reserve_ex(cache_, p, ints(3), l, 3, ints(1), work),
+             lambda p, l: qi.kv_pages_fork_ex(cache_, p, l, ints(3), 3, ints(1), work), lambda p, l: qi.kv_pages_fork_ex(cache_, p, ints(3), l, 3, ints(1), work),
+             lambda p, l: qi.kv_pages_free_ex(cache_, p, l, 3)]
+    for call in calls:
+        for bad in (ints(2), ints(3).long(), ints(6)[::2], torch.zeros(3), ints(3).to("meta")):
+            with pytest.raises(ValueError):
+                call(pages_, bad)
+        for unfit in [few] + elsewhere:
+            with pytest.raises(ValueError):
+                call(unfit, ints(3))
+    copies = [lambda l: qi.kv_pages_copy_ex(cache_, l, ints(3), 3), lambda l: qi.kv_pages_copy_ex(cache_, ints(3), l, 3)]
+    for call in copies:
+        for bad in (ints(2), ints(3).long()):
+            with pytest.raises(ValueError):
+                call(bad)
+    for word in (ints(0), ints(1).long()):
+        with pytest.raises(ValueError):
+            qi.kv_pages_compact_ex(cache_, pages_, word, work)
+        with pytest.raises(ValueError):
+            qi.kv_pages_reserve_ex(cache_, pages_, ints(3), ints(3), 3, word, work)
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    for call in (lambda: qi.kv_append_ex(cache_, few, batch_, 0, x, x, qi.DTYPE_F16, 128, 128), lambda: qi.kv_read_ex(cache_, few, batch_, 0, x, x, qi.DTYPE_F16, 128, 128),
+                 lambda: qi.kv_attention_ex(cache_, few, batch_, 0, x, 128, x, 128, 2, 1.0, 160, workspace=work), lambda: qi.kv_pages_compact_ex(cache_, few, ints(1), work),
+                 lambda: qi.kv_append_ex(cache_, pages_, qi.KvBatch(None, ints(3).to("meta"), 4, 2), 0, x, x, qi.DTYPE_F16, 128, 128),
+                 lambda: qi.kv_attention_ex(cache_, pages_, qi.KvBatch(ints(2).to("meta"), ints(3), 4, 2), 0, x, 128, x, 128, 2, 1.0, 160, workspace=work)):
+        with pytest.raises(ValueError):
+            call()
