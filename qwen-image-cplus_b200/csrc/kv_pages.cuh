@@ -97,8 +97,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(PageTables t, con
         int need = 0;
         if (i < n) {
             const int slot = slots[i], count = counts[i];
-            if (!known(t, slot) || count < 0 || t.lengths[slot] < 0 || count > 0x7fffffff - t.lengths[slot] || pages_of(t.lengths[slot] + count, t.page_shift) > t.table_pages) wrong = 1;
-            else need = pages_of(t.lengths[slot] + count, t.page_shift) - pages_of(t.lengths[slot], t.page_shift);
+            if (!known(t, slot) || count < 0 || t.lengths[slot] < 0 || count > 0x7fffffff - t.lengths[slot] || pages_of(t.lengths[slot] + count, t.page_shift) > t.table_pages) {
+                wrong = 1;
+            } else {
+                work.held[i] = t.lengths[slot];
+                need = pages_of(work.held[i] + count, t.page_shift) - pages_of(work.held[i], t.page_shift);
+            }
         }
         int total;
         const int before = scan_before(need, warp_sums, total);
@@ -114,10 +118,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) reserve_kernel(PageTables t, con
     const int found = collect<false>(t.references, 0, t.pages, wanted, work.moved, warp_sums);
     if (threadIdx.x == 0) *shortage = wanted - found;
     if (found < wanted) return;
-    // A warp takes a sequence: short ones (one new token each) and long ones (a prompt) alike
+    // A warp takes a sequence: short ones (one new token each) and long ones (a prompt) alike. Its length is the one that was checked, so
+    // that a sequence that is named twice, against the rules, does not grow beyond its row or its share of the pages.
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < n; i += PLAN_THREADS / 32) {
-        const int slot = slots[i], length = t.lengths[slot], more = counts[i];
+        const int slot = slots[i], length = work.held[i], more = counts[i];
         const int have = pages_of(length, t.page_shift), want = pages_of(length + more, t.page_shift), first = work.sources[i];
         for (int j = have + lane; j < want; j += 32) t.table[static_cast<long long>(slot) * t.table_pages + j] = work.moved[first + j - have];
         __syncwarp();

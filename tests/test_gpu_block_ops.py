@@ -661,6 +661,30 @@ def test_pages_that_do_not_suffice_change_nothing(qi):
     ledger.check(start)
 
 
+def test_reserving_for_a_sequence_twice_stays_within_its_row(qi):
+    # against the rules, and what it gives is not defined, but other rows, what lies behind the table and other pages are left alone
+    page, sequences, width = 16, 40, 3
+    store = Store(qi, 41, [32] * sequences, page=page, spare=50, table_extra=1)
+    whole = torch.full((sequences * width + 64,), 1234567, dtype=torch.int32, device="cuda")
+    whole[: sequences * width] = store.table.flatten()
+    table = whole[: sequences * width].view(sequences, width)
+    pages = qi.KvPages(table, store.lengths, store.references)
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, pages), dtype=torch.uint8, device="cuda").fill_(0xA5)
+    told, last = ints([0]), sequences - 1
+    slots = [last] + list(range(31)) + [last] + [31, 32]  # the first and the 33rd of the list are one warp's, one after the other
+    assert qi.kv_pages_reserve_ex(store.cache, pages, ints(slots), ints([16] * len(slots)), len(slots), told, workspace) == 0
+    settled(qi)
+    assert told.item() == 0
+    assert (whole[sequences * width:] == 1234567).all()
+    assert ((table >= -1) & (table < len(store.references))).all() and (store.lengths <= width * page).all()
+    for s in range(33):
+        assert store.lengths[s] == 48 and table[s, 2] >= 0
+    for s in range(33, last):
+        assert store.lengths[s] == 32 and table[s, 2] == -1
+    held = table[table >= 0]
+    assert len(held.unique()) == len(held)
+
+
 def test_pages_of_a_large_pool(qi):
     # more pages than one round of the planning CTA looks at, and a compaction that moves most of them
     store = Store(qi, 6, [16 * 9] * 700, page=16, layers=1, layer=0, kv_heads=1, head_dim=64, spare=6000, table_extra=2)
