@@ -90,7 +90,7 @@ __device__ __forceinline__ uint4 load_codes(const uint8_t *at) {  // read once b
 }
 // Quotients of what may need 64 bits but hardly ever does.
 __device__ __forceinline__ long long divide(long long a, long long b) {
-    if (static_cast<unsigned long long>(a) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    if (static_cast<unsigned long long>(a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
     return a / b;
 }
 

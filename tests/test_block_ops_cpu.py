@@ -1,6 +1,8 @@
 """What the operators between the packed linears refuse before anything is launched, and their plans; no GPU needed."""
 import ctypes
 import os
+import re
+import subprocess
 
 import pytest
 
@@ -251,3 +253,15 @@ def test_lists_and_pools_that_are_too_short(qi):
                  lambda: qi.kv_attention_ex(cache_, pages_, qi.KvBatch(ints(2).to("meta"), ints(3), 4, 2), 0, x, 128, x, 128, 2, 1.0, 160, workspace=work)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_quotients_that_need_64_bits(tmp_path):
+    # the kernel's own function, compiled for the host: which CTA has a round when there are more rounds than 32 bits count
+    source = open(os.path.join(entry.PACKAGE_DIR, "csrc", "kv_decode.cuh"), encoding="utf-8").read()
+    body = re.search(r"__device__ __forceinline__ (long long divide\(.*?\n}\n)", source, re.S).group(1)
+    pairs = [(a, b) for a in (0, 1, 295, 296, 2 ** 31, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 5, 2 ** 40 + 7) for b in (1, 3, 296, 2 ** 31, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 2, 3 * 2 ** 33)]
+    checks = "".join(f"if (divide({a}LL, {b}LL) != {a // b}LL) return {i + 1};" for i, (a, b) in enumerate(pairs))
+    program = tmp_path / "divide.cpp"
+    program.write_text("#include <cstdint>\nstatic " + body + "int main() { " + checks + " return 0; }\n")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "divide"), str(program)], check=True)
+    assert subprocess.run([str(tmp_path / "divide")]).returncode == 0
