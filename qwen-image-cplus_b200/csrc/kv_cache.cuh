@@ -129,6 +129,14 @@ __device__ __forceinline__ void load_values(const T *source, float (&x)[16 / siz
     }
 }
 
+// The larger one in magnitude; NaN where either is.
+__device__ __forceinline__ float larger_or_nan(float peak, float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(peak), "f"(fabsf(x)));
+    return y;
+}
+
+constexpr uint32_t INFINITE = 0x7f800000u;  // as bits: NaN's are above
 constexpr float ROUND_MAGIC = 12582912.0f, NEAR_TIE = 0.5f - 1.0f / 16384.0f, LEAST_NORMAL_SCALE = 1e-36f;
 
 template <typename T, int DIM>
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) append_kernel(Cache cache, Ta
     const T *source = (u.which == 0 ? k : v) + static_cast<long long>(u.head) * DIM + channel;
     const long long ld = u.which == 0 ? ld_k : ld_v, row0 = u.entry.first + static_cast<long long>(u.block) * BLOCK - u.start;
     float x[PASSES][CHANNELS];
-    float peak = 0.0f;
+    float peak;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int token = i * TOKENS + within;
@@ -152,11 +160,25 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) append_kernel(Cache cache, Ta
     }
     if (!place_unit(cache, tables, DIM, true, 0xC001, u)) return;
     const float old = u.early > 0 ? *u.scale : 0.0f;
+    // no negative ones: ordered as whole numbers
+    auto largest = [&]() {
+        peak = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i)
+        for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-        for (int j = 0; j < CHANNELS; ++j) peak = fmaxf(peak, fabsf(x[i][j]));
-    peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));  // no negative ones: ordered as whole numbers
+            for (int j = 0; j < CHANNELS; ++j) peak = larger_or_nan(peak, x[i][j]);
+        peak = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)));
+    };
+    largest();
+    if (__float_as_uint(peak) >= INFINITE) {  // what no scale could hold is 0, and its neighbours stay what they are
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+            for (int j = 0; j < CHANNELS; ++j)
+                if ((__float_as_uint(x[i][j]) & INFINITE) == INFINITE) x[i][j] = 0.0f;
+        largest();
+        if (lane == 0) complain(0xC002);
+    }
     const float scale = fmaxf(old, __fmul_rn(peak, 1.0f / 127.0f));
     if (u.early > 0 && scale > old) {
         const float factor = __fdiv_rn(old, scale);

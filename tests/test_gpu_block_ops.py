@@ -502,6 +502,28 @@ def test_append_and_read_without_a_bound_of_new_tokens(qi, kv_heads):
         assert torch.equal(out[i].view(expected.shape), expected)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_append_holds_what_is_not_finite_as_zero_and_says_so(qi, dtype, head_dim):
+    lengths, counts = [1, 60, 333], [1, 41, 300]
+    code = qi.DTYPE_F16 if dtype == torch.float16 else qi.DTYPE_F32
+    a, b = (Store(qi, 43, lengths, head_dim=head_dim) for _ in range(2))
+    rows, kv = make_kv(a, sum(counts), dtype, 44)
+    width, g = a.kv_heads * head_dim, random.Random(45)
+    places = [(0, 3), (1, width), (17, 2 * width - 1), (18, 0), (18, 1)] + [(g.randrange(20, 342), g.randrange(2 * width)) for _ in range(60)]
+    places += [(200, c) for c in range(2 * width)]  # a token of nothing else
+    clean = rows.clone()
+    for i, (token, channel) in enumerate(places):
+        rows[token, channel], clean[token, channel] = (float("nan"), float("inf"), float("-inf"))[i % 3], 0.0
+    append_plain(b, {"k": clean[:, :width].reshape(-1, a.kv_heads, head_dim), "v": clean[:, width:].reshape(-1, a.kv_heads, head_dim)}, [0, 1, 2], counts)
+    for _ in range(2):
+        assert qi.kv_append_ex(a.cache, a.pages, a.batch([0, 1, 2], counts), 1, rows, rows[:, width:], code, 2 * width, 2 * width) == 0
+        assert qi.kernel_status() & 0xfffff == 0x6C002
+        assert same_bytes(a, b)
+    assert qi.kv_append_ex(a.cache, a.pages, a.batch([0, 1, 2], counts), 1, clean, clean[:, width:], code, 2 * width, 2 * width) == 0
+    settled(qi)
+
+
 def test_append_leaves_shared_and_missing_pages_alone(qi):
     # page numbers are the device's own: what must not be written is left as it is, and the status word says so
     for fault in ("shared", "missing", "foreign", "count", "slot"):
