@@ -61,30 +61,35 @@ class Server:
         self.cache = qi.KvCache(torch.empty(*shape, **byte), torch.empty(*shape, **byte), torch.empty(*scales, device="cuda"), torch.empty(*scales, device="cuda"))
         self.pages = qi.KvPages(torch.full((SEQUENCES, -(-LONGEST // PAGE)), -1, dtype=torch.int32, device="cuda"), ints([0] * SEQUENCES), ints([0] * PAGES))
         self.page_work = torch.empty(qi.kv_pages_workspace(self.cache, self.pages), **byte)
-        self.told = ints([0])
+        self.words, self.used, self.room = [], ints([0]), None  # what reservations and forks told, a word each: nothing waits for it
         bounds = [qi.KvBatch(ints([0]), ints([0, n]), n, n) for n in (1, LONGEST)]
         bounds += [qi.KvBatch(ints([0] * SEQUENCES), ints([0] * (SEQUENCES + 1)), SEQUENCES, 1)]
         self.attention_work = torch.zeros(max(qi.kv_attention_workspace(self.cache, b, HEADS, LONGEST) for b in bounds), **byte)
         self.work = qi.LinearWork(torch.empty(LONGEST, MLP // 2, **byte), torch.empty(LONGEST, MLP // 64, dtype=torch.float16, device="cuda"),
                                   torch.empty(LONGEST, MLP, dtype=torch.float16, device="cuda"), torch.empty(LONGEST, MLP, **byte))
 
+    def word(self):
+        self.words.append(ints([0]))
+        return self.words[-1]
+
     def reserve(self, slots, counts):
-        ok(self.qi.kv_pages_reserve_ex(self.cache, self.pages, ints(slots), ints(counts), len(slots), self.told, self.page_work))
+        self.room = self.word()  # forward() leaves the cache alone where there is none
+        ok(self.qi.kv_pages_reserve_ex(self.cache, self.pages, ints(slots), ints(counts), len(slots), self.room, self.page_work))
 
     def fork(self, parent, child):
-        ok(self.qi.kv_pages_fork_ex(self.cache, self.pages, ints([parent]), ints([child]), 1, self.told, self.page_work))
+        ok(self.qi.kv_pages_fork_ex(self.cache, self.pages, ints([parent]), ints([child]), 1, self.word(), self.page_work))
 
     def end(self, slot):
         ok(self.qi.kv_pages_free_ex(self.cache, self.pages, ints([slot]), 1))
 
     def compact(self):
-        ok(self.qi.kv_pages_compact_ex(self.cache, self.pages, self.told, self.page_work))
+        ok(self.qi.kv_pages_compact_ex(self.cache, self.pages, self.used, self.page_work))
 
     def forward(self, slots, counts, tokens):
         """The hidden states of `tokens` [sum(counts), WIDTH], which are the last counts[i] tokens of sequence slots[i]."""
         qi, rows = self.qi, sum(counts)
         half = dict(dtype=torch.float16, device="cuda")
-        batch = qi.KvBatch(ints(slots), ints([sum(counts[:i]) for i in range(len(counts) + 1)]), rows, max(counts))
+        batch = qi.KvBatch(ints(slots), ints([sum(counts[:i]) for i in range(len(counts) + 1)]), rows, max(counts), self.room)
         residual, x = tokens.clone(), torch.empty(rows, WIDTH, **half)
         qkv, y, out, hidden = torch.empty(rows, QKV, **half), torch.empty(rows, HEADS * HEAD_DIM, **half), torch.empty(rows, WIDTH, **half), torch.empty(rows, MLP, **half)
 
@@ -131,8 +136,8 @@ def main():
     server.reserve([1], [count])
     at_once = server.forward([1], [count], tokens[:count])[-1:]
     torch.cuda.synchronize()
-    if qi.kernel_status() != 0 or server.told.item() != 0:
-        raise RuntimeError("a call found something unsound")
+    if qi.kernel_status() != 0 or any(word.item() != 0 for word in server.words):
+        raise RuntimeError("a call found something unsound, or no room")
     difference = ((last - at_once).float().norm() / at_once.float().norm()).item()
     print(f"{LAYERS} blocks, {count} tokens: {server.pages.lengths.tolist()} tokens held, {int((server.pages.references > 0).sum())} pages in use, "
           f"step by step against at once: {difference:.1e} apart")

@@ -457,10 +457,13 @@ typedef struct {
 
 /* A ragged batch: entry b is the LAST offsets[b + 1] - offsets[b] tokens of sequence slots[b] (slots NULL: of sequence b),
  * whose rows begin at row offsets[b] of the token arrays. offsets[0] = 0; `tokens` rows in all and `most` for one entry are
- * bounds that the host knows; entries <= 65535. No sequence may be named twice where a call writes. */
+ * bounds that the host knows; entries <= 65535. No sequence may be named twice where a call writes.
+ * shortage: what a reservation of these tokens told (device), or NULL. Where it is not 0 when the call runs, the call does nothing, for lengths
+ * do not count the tokens then: append would write them over earlier ones. */
 typedef struct {
     const int *slots, *offsets;
     int entries, tokens, most;
+    const int *shortage;
 } qi_kv_batch;
 
 /* Writes new tokens into layer `layer`: row r of k and v [tokens, kv_heads, head_dim], ld_k and ld_v elements between rows
@@ -511,7 +514,8 @@ int qi_kv_pages_workspace(const qi_kv_cache *cache, const qi_kv_pages *pages, si
 
 /* Pages for counts[i] more tokens of sequence slots[i], whose length grows by them: for all of the list, or for none when too few
  * pages are free. *shortage (device) becomes 0, how many pages are missing, or -1 where the list itself is at fault (an unknown
- * sequence, or one too long for its row of the table). No sequence twice. */
+ * sequence, or one too long for its row of the table). No sequence twice. Whoever does not wait for the word names it in the batches of the
+ * tokens (qi_kv_batch) and gives each step one of its own, or the next call's overwrites it. */
 int qi_kv_pages_reserve_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const int *slots, const int *counts, int n,
                            int *shortage, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -100,7 +100,7 @@ class qi_kv_pages(ctypes.Structure):
 
 class qi_kv_batch(ctypes.Structure):
     _fields_ = [("slots", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("entries", ctypes.c_int), ("tokens", ctypes.c_int),
-                ("most", ctypes.c_int)]
+                ("most", ctypes.c_int), ("shortage", ctypes.c_void_p)]
 
 
 class qi_kv_attention(ctypes.Structure):
@@ -521,15 +521,16 @@ class KvPages:
 
 
 class KvBatch:
-    """The last offsets[b + 1] - offsets[b] tokens of sequence slots[b] (None: b) for each entry; `tokens` rows, at most `most` for one."""
+    """The last offsets[b + 1] - offsets[b] tokens of sequence slots[b] (None: b) for each entry; `tokens` rows, at most `most` for one.
+    `shortage`: the word that told whether there was room for them; calls do nothing where there was not."""
 
-    def __init__(self, slots, offsets, tokens: int, most: int):
-        self.slots, self.offsets = slots, offsets
+    def __init__(self, slots, offsets, tokens: int, most: int, shortage=None):
+        self.slots, self.offsets, self.shortage = slots, offsets, shortage
         entries = offsets.numel() - 1
-        self.lists = (offsets,) if slots is None else (offsets, slots)
-        if entries < 0 or not _are("int32", *self.lists) or (slots is not None and slots.numel() < entries):
-            raise ValueError("a batch has contiguous int32: an offset more than entries, and a slot for each")
-        self.batch = qi_kv_batch(_p(slots), _p(offsets), entries, tokens, most)
+        self.lists = tuple(t for t in (offsets, slots, shortage) if t is not None)
+        if entries < 0 or not _are("int32", *self.lists) or (slots is not None and slots.numel() < entries) or (shortage is not None and shortage.numel() < 1):
+            raise ValueError("a batch has contiguous int32: an offset more than entries, a slot for each, and a word that tells of a shortage")
+        self.batch = qi_kv_batch(_p(slots), _p(offsets), entries, tokens, most, _p(shortage))
         self.reference = ctypes.byref(self.batch)
         self.pool = None  # the one that it has been found beside
 

@@ -39,7 +39,7 @@ bool sound(const qi_kv_pages *pages) {
            pages->sequences > 0 && pages->table_pages > 0 && pages->table_pages <= kv::MOST_TABLE_PAGES;
 }
 bool sound(const qi_kv_batch *batch) {
-    return batch && batch->offsets && aligned4(batch->offsets) && aligned4(batch->slots) && batch->entries >= 0 && batch->entries <= 65535 && batch->tokens >= 0 && batch->most >= 0;
+    return batch && batch->offsets && aligned4(batch->offsets) && aligned4(batch->slots) && aligned4(batch->shortage) && batch->entries >= 0 && batch->entries <= 65535 && batch->tokens >= 0 && batch->most >= 0;
 }
 
 kv::Cache layer_of(const qi_kv_cache *cache, int layer) {
@@ -51,7 +51,7 @@ kv::Cache layer_of(const qi_kv_cache *cache, int layer) {
     return c;
 }
 kv::Tables tables_of(const qi_kv_pages *pages) { return {pages->table, pages->lengths, pages->references, pages->sequences, pages->table_pages}; }
-kv::Batch batch_of(const qi_kv_batch *batch) { return {batch->slots, batch->offsets, batch->entries, batch->tokens, batch->most}; }
+kv::Batch batch_of(const qi_kv_batch *batch) { return {batch->slots, batch->offsets, batch->entries, batch->tokens, batch->most, batch->shortage}; }
 
 // A launch of any grid, overlapped with the kernel before it.
 template <typename... Parameters, typename... Arguments>

@@ -34,6 +34,7 @@ struct Tables {
 struct Batch {
     const int *slots, *offsets;
     int entries, tokens, most;
+    const int *shortage;
 };
 
 // One entry of a batch: the last `count` tokens of a sequence of `length` tokens, `first` of the batch's token rows on.
@@ -42,6 +43,9 @@ struct Entry {
 };
 
 __device__ __forceinline__ void complain(uint32_t detail) { atomicCAS(&g_status, 0u, STATUS_BAD_ARGUMENT | detail); }
+
+// The batch's tokens have no pages, and lengths do not count them.
+__device__ __forceinline__ bool no_room(const Batch &batch) { return batch.shortage != nullptr && __ldg(batch.shortage) != 0; }
 
 // What the host cannot check without waiting for the device is checked here, by every CTA: nothing is read or written through
 // an entry that is not sound, and the status word says so.
@@ -85,6 +89,7 @@ struct Unit {
 
 // Which tokens of which block; false: nothing to do, or nothing that may be done.
 __device__ __forceinline__ bool read_unit(const Cache &cache, const Tables &tables, const Batch &batch, uint32_t detail, Unit &u) {
+    if (no_room(batch)) return false;
     const int unit = blockIdx.x * UNIT_WARPS + (threadIdx.x >> 5);  // (block, head, keys or values)
     u.which = unit & 1, u.head = (unit >> 1) % cache.heads;
     const bool sound = read_entry(batch, tables, cache.page_shift, blockIdx.y, 0x7fffffff, u.entry);

@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
     __shared__ long long warp_rounds[DECODE_WARPS], first_before, bounds[2];
     __shared__ int warp_entries[DECODE_WARPS], warp_longest[DECODE_WARPS];
     grid_wait();
+    if (no_room(batch)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row8 = lane >> 2, quad = lane & 3;
 
     // ---- which rounds are this CTA's ----

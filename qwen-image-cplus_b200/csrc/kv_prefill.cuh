@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(PREFILL_THREADS, 1) prefill_kernel(Cache cache
     Entry entry;
     const bool sound = read_entry(batch, tables, cache.page_shift, b, a.max_length, entry);
     if (!sound && threadIdx.x == 0) complain(0xC040);
-    const int rows = sound ? entry.count * a.group : 0, first_row = tile * PREFILL_ROWS;
+    const int rows = sound && !no_room(batch) ? entry.count * a.group : 0, first_row = tile * PREFILL_ROWS;
     const int last_row = min(first_row + PREFILL_ROWS, rows) - 1;
     int low = 0, high = 0, unused, used = 0;
     if (first_row < rows) {

@@ -215,6 +215,11 @@ def test_structures_of_other_types_and_sizes(qi):
     for parts in ((slots, offsets.long()), (slots.long(), offsets), (slots[:2], offsets), (None, offsets[:0]), (None, offsets.float()), (torch.zeros(6, dtype=torch.int32)[::2], offsets)):
         with pytest.raises(ValueError):
             qi.KvBatch(*parts, 5, 2)
+    for word in (torch.zeros(1), torch.zeros(1, dtype=torch.int64), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            qi.KvBatch(slots, offsets, 5, 2, word)
+    for status in every_call(qi, cache(qi), pages(qi), batch(qi, shortage=258)):
+        assert status == INVALID
     qi.KvBatch(None, offsets, 5, 2), qi.KvBatch(slots, offsets, 5, 2), qi.KvBatch(torch.zeros(9, dtype=torch.int32), offsets, 5, 2)
 
 

@@ -660,6 +660,47 @@ def test_pages_follow_the_ledger(qi, seed, page, layers, kv_heads, head_dim):
         ledger.check(start)
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [5, 1], [60, 33]])
+def test_a_step_without_room_leaves_the_cache_alone(qi, counts):
+    # the calls of a step are queued behind its reservation without waiting for it; where that falls short, "the last tokens" are earlier ones
+    page, heads, dim = 16, 4, 128
+    lengths = [32, 64, 80, 16]
+    store, before = (Store(qi, 47, lengths, page=page, spare=1, table_extra=8) for _ in range(2))
+    workspace = torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda")
+    told, tokens = ints([5]), sum(counts)
+    batch = qi.KvBatch(ints([0, 1]), ints([0, counts[0], tokens]), tokens, max(counts), told)
+    rows, kv = make_kv(store, tokens, torch.float16, 48)
+    q = (torch.randn(tokens, heads, dim, device="cuda") * 1.5).half()
+    work = torch.zeros(max(qi.kv_attention_workspace(store.cache, batch, heads, 200), 16), dtype=torch.uint8, device="cuda")
+
+    def step():
+        y, lse, out = torch.full_like(q, float("nan")), torch.full((tokens, heads), float("nan"), device="cuda"), torch.full((2, tokens, 2, dim), float("nan"), device="cuda")
+        assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints([0, 1]), ints(counts), 2, told, workspace) == 0
+        assert qi.kv_append_ex(store.cache, store.pages, batch, 1, rows, rows[:, 256:], qi.DTYPE_F16, 512, 512) == 0
+        assert qi.kv_attention_ex(store.cache, store.pages, batch, 1, q, heads * dim, y, heads * dim, heads, dim ** -0.5, 200, lse=lse, workspace=work) == 0
+        assert qi.kv_read_ex(store.cache, store.pages, batch, 1, out[0], out[1], qi.DTYPE_F32, 2 * dim, 2 * dim) == 0
+        settled(qi)
+        return y, lse, out
+
+    y, lse, out = step()
+    assert told.item() > 0 and store.lengths.tolist() == lengths
+    assert same_bytes(store, before) and y.isnan().all() and lse.isnan().all() and out.isnan().all()
+    told.fill_(-1)  # a list at fault likewise
+    assert qi.kv_append_ex(store.cache, store.pages, batch, 1, rows, rows[:, 256:], qi.DTYPE_F16, 512, 512) == 0
+    settled(qi)
+    assert same_bytes(store, before)
+    assert qi.kv_pages_free_ex(store.cache, store.pages, ints([2, 3]), 2) == 0
+    y, lse, out = step()
+    assert told.item() == 0
+    store.lengths_list = before.lengths_list = [32 + counts[0], 64 + counts[1], 0, 0]
+    before.table.copy_(store.table)
+    append_plain(before, kv, [0, 1], counts)
+    assert same_bytes(store, before)
+    exact, _ = attend_exact(store, q, [0, 1], counts, heads, dim ** -0.5, True, 0)
+    assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm()
+    assert torch.equal(out[0], torch.cat([store.values("k", s)[-n:] for s, n in zip((0, 1), counts)]).float())
+
+
 def test_pages_that_do_not_suffice_change_nothing(qi):
     store = Store(qi, 5, [40, 64, 33], page=32, spare=1, table_extra=4)
     ledger, start = Ledger(store), pool_copy(store)
