@@ -62,9 +62,8 @@ class Server:
         self.pages = qi.KvPages(torch.full((SEQUENCES, -(-LONGEST // PAGE)), -1, dtype=torch.int32, device="cuda"), ints([0] * SEQUENCES), ints([0] * PAGES))
         self.page_work = torch.empty(qi.kv_pages_workspace(self.cache, self.pages), **byte)
         self.words, self.used, self.room = [], ints([0]), None  # what reservations and forks told, a word each: nothing waits for it
-        bounds = [qi.KvBatch(ints([0]), ints([0, n]), n, n) for n in (1, LONGEST)]
-        bounds += [qi.KvBatch(ints([0] * SEQUENCES), ints([0] * (SEQUENCES + 1)), SEQUENCES, 1)]
-        self.attention_work = torch.zeros(max(qi.kv_attention_workspace(self.cache, b, HEADS, LONGEST) for b in bounds), **byte)
+        most = qi.KvBatch(None, ints([0] * (SEQUENCES + 1)), SEQUENCES * LONGEST, LONGEST)  # no step is larger
+        self.attention_work = torch.zeros(qi.kv_attention_workspace(self.cache, most, HEADS, LONGEST), **byte)
         self.work = qi.LinearWork(torch.empty(LONGEST, MLP // 2, **byte), torch.empty(LONGEST, MLP // 64, dtype=torch.float16, device="cuda"),
                                   torch.empty(LONGEST, MLP, dtype=torch.float16, device="cuda"), torch.empty(LONGEST, MLP, **byte))
 

@@ -490,9 +490,10 @@ int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
  * joined. Queries and weights enter the products as float16, codes exactly; all sums are float32. Tokens whose
  * page the table does not name soundly are hidden from all rows, an entry that is unsound leaves its rows of y and lse as they are, and the status word says so. max_length bounds the
  * lengths of the batch's sequences (0x7fffffff: whatever the table holds).
- * workspace: qi_kv_attention_workspace() bytes (0: none needed) for the same cache, batch bounds, heads and max_length, 16-byte
- * aligned, zeroed once before its first use; every call leaves its counters zero. Calls of any shapes that it is large enough for may share
- * it, one at a time. most * (heads / kv_heads) / 256 * kv_heads, rounded up, is at most 65535 where most * (heads / kv_heads) > 16. */
+ * workspace: 16-byte aligned, zeroed once before its first use; every call leaves its counters zero. qi_kv_attention_workspace() gives the bytes (0: none
+ * needed) that serve every call on the same cache with as many heads whose entries, `most` and max_length are no larger, with any window. Calls of any
+ * shapes that it is large enough for may share it, one
+ * at a time. most * (heads / kv_heads) / 256 * kv_heads, rounded up, is at most 65535 where most * (heads / kv_heads) > 16. */
 typedef struct {
     int layer, heads;
     const void *q;

@@ -558,7 +558,7 @@ def _bytes_of(workspace) -> int:
 
 
 def kv_attention_workspace(cache: KvCache, batch: KvBatch, heads: int, max_length: int) -> int:
-    """Bytes of workspace (to be zeroed once) that kv_attention_ex needs for batches within these bounds."""
+    """Bytes of workspace (to be zeroed once) with which kv_attention_ex takes every batch of no more entries, no larger `most` and no longer sequences."""
     value = ctypes.c_size_t(0)
     status = lib().qi_kv_attention_workspace(cache.reference, batch.reference, heads, max_length, ctypes.byref(value))
     if status != 0:

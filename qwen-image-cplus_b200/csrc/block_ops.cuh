@@ -112,21 +112,32 @@ constexpr int DECODE_ROWS = 16;
 // A bound of lengths, cut to the tokens of a row of the table: at most 2^27, so that no piece of it leaves int and a loose bound costs nothing.
 int held_length(const qi_kv_cache *cache, int table_pages, int max_length) { return std::min(max_length, table_pages * cache->page_tokens); }
 
+// CTAs of the streaming kernel, and its workspace. One counter for each of its CTAs, or for each tile of rows that is cut into pieces (at most half as
+// many as SMs), lies at the same place for every call, so that calls of different shapes may share a workspace.
+size_t counter_bytes(int sms) { return (static_cast<size_t>(sms) * 3 * 4 + 255) / 256 * 256; }
+int streaming_grid(const qi_kv_cache *cache, int tiles, int sms) {
+    return sms * (cache->head_dim == 128 ? (tiles == 1 ? kv::Decode<128, 1>::CTAS : kv::Decode<128, 2>::CTAS) : (tiles == 1 ? kv::Decode<64, 1>::CTAS : kv::Decode<64, 2>::CTAS));
+}
+size_t streaming_bytes(const qi_kv_cache *cache, int tiles, int max_length, int sms) {  // units of one round each are never shared
+    return max_length <= kv::ROUND ? 0 : counter_bytes(sms) + static_cast<size_t>(streaming_grid(cache, tiles, sms)) * 2 * (8 * tiles) * (cache->head_dim + 2) * 4;
+}
+// The workspace of so many tiles of rows, with room for as many pieces as any window gives.
+size_t piece_bytes(const qi_kv_cache *cache, long long units, int max_length, int sms) {
+    const long long most = std::min(sms / units, (max_length + kv::TILE_TOKENS - 1LL) / kv::TILE_TOKENS);
+    return most > 1 ? counter_bytes(sms) + static_cast<size_t>(units) * most * kv::PREFILL_ROWS * (cache->head_dim + 2) * 4 : 0;
+}
+
 // How a call is cut. The streaming kernel shares the tokens out by itself. The other one takes a CTA to a tile of rows, one to an SM, and
 // where there are too few tiles for the GPU, several to pieces of its tokens.
 bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int window, int sms, AttentionPlan &plan) {
     if (heads <= 0 || heads % cache->kv_heads != 0 || max_length < 0 || window < 0) return false;
     const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads), entries = batch->entries > 0 ? batch->entries : 1;
     plan.tiles = rows <= 8 ? 1 : rows <= DECODE_ROWS ? 2 : 0;
-    // One counter for each CTA of the streaming kernel or each tile of rows that is cut into pieces (at most half as many as SMs), at the same place
-    // for every call, so that calls of different shapes may share a workspace
-    plan.partial_offset = (static_cast<size_t>(sms) * 3 * 4 + 255) / 256 * 256;
-    plan.grid = sms * (cache->head_dim == 128 ? (plan.tiles == 1 ? kv::Decode<128, 1>::CTAS : kv::Decode<128, 2>::CTAS)
-                                              : (plan.tiles == 1 ? kv::Decode<64, 1>::CTAS : kv::Decode<64, 2>::CTAS));
+    plan.partial_offset = counter_bytes(sms);
+    plan.grid = streaming_grid(cache, plan.tiles, sms);
     plan.row_tiles = 1, plan.chunk = 0, plan.splits = 1;
     if (plan.tiles > 0) {
-        // units of one round each are never shared
-        plan.bytes = max_length <= kv::ROUND ? 0 : plan.partial_offset + static_cast<size_t>(plan.grid) * 2 * (8 * plan.tiles) * (cache->head_dim + 2) * 4;
+        plan.bytes = streaming_bytes(cache, plan.tiles, max_length, sms);
         return true;
     }
     const long long row_tiles = (rows + kv::PREFILL_ROWS - 1) / kv::PREFILL_ROWS;
@@ -140,9 +151,20 @@ bool plan_attention(const qi_kv_cache *cache, const qi_kv_batch *batch, int head
     chunk = (chunk + kv::TILE_TOKENS - 1) / kv::TILE_TOKENS * kv::TILE_TOKENS;
     if (chunk < kv::TILE_TOKENS) chunk = kv::TILE_TOKENS;
     plan.chunk = static_cast<int>(chunk), plan.splits = static_cast<int>(span > 0 ? (span + chunk - 1) / chunk : 1);
-    // room for as many pieces as any window gives
-    const long long most = std::min(pieces, (max_length + kv::TILE_TOKENS - 1LL) / kv::TILE_TOKENS);
-    plan.bytes = most > 1 ? plan.partial_offset + static_cast<size_t>(units) * most * kv::PREFILL_ROWS * (cache->head_dim + 2) * 4 : 0;
+    plan.bytes = piece_bytes(cache, units, max_length, sms);
+    return true;
+}
+
+// What any call within the bounds of `batch` and `max_length` needs: few tiles of rows are cut into pieces, so a smaller call can need more.
+bool attention_bytes(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, int sms, size_t &bytes) {
+    AttentionPlan plan;
+    if (!plan_attention(cache, batch, heads, max_length, 0, sms, plan)) return false;
+    bytes = std::max(plan.bytes, streaming_bytes(cache, 1, max_length, sms));
+    const long long rows = static_cast<long long>(batch->most) * (heads / cache->kv_heads);
+    if (rows > 8) bytes = std::max(bytes, streaming_bytes(cache, 2, max_length, sms));
+    if (plan.tiles == 0)
+        for (long long units = cache->kv_heads; units <= std::min(static_cast<long long>(plan.row_tiles) * cache->kv_heads * std::max(batch->entries, 1), sms / 2LL); units += cache->kv_heads)
+            bytes = std::max(bytes, piece_bytes(cache, units, max_length, sms));
     return true;
 }
 
@@ -237,9 +259,7 @@ int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
 }
 
 int qi_kv_attention_workspace(const qi_kv_cache *cache, const qi_kv_batch *batch, int heads, int max_length, size_t *bytes) {
-    AttentionPlan plan;
-    if (!sound(cache) || !sound(batch) || !bytes || !plan_attention(cache, batch, heads, held_length(cache, kv::MOST_TABLE_PAGES, max_length), 0, sms_or_usual(), plan)) return INVALID;
-    *bytes = plan.bytes;
+    if (!sound(cache) || !sound(batch) || !bytes || !attention_bytes(cache, batch, heads, held_length(cache, kv::MOST_TABLE_PAGES, max_length), sms_or_usual(), *bytes)) return INVALID;
     return 0;
 }
 

@@ -156,6 +156,29 @@ def test_attention_refuses_a_workspace_that_is_too_small(qi):
         assert without_a_device(library.qi_kv_attention_ex(ctypes.byref(c), ctypes.byref(p), ctypes.byref(b), ctypes.byref(call), 256, size.value, None))
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("kv_heads,heads", [(4, 32), (1, 1), (8, 24), (32, 32), (80, 80), (2, 40)])
+def test_a_workspace_for_the_largest_batch_serves_the_smaller_ones(qi, kv_heads, heads, head_dim):
+    torch = pytest.importorskip("torch")
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    library, c, p = qi.lib(), cache(qi, kv_heads=kv_heads, head_dim=head_dim), pages(qi, table_pages=400)
+    size, width = ctypes.c_size_t(0), heads * head_dim
+    for entries, most, length in ((8, 4096, 8192), (70, 12, 5000), (3, 300, 700), (64, 1, 8192), (1, 40, 12800), (5, 2, 128)):
+        assert library.qi_kv_attention_workspace(ctypes.byref(c), ctypes.byref(batch(qi, entries=entries, tokens=entries * most, most=most)), heads, length, ctypes.byref(size)) == 0
+        bound = size.value
+        for fewer in sorted({1, 2, 7, entries // 2, entries - 1, entries}):
+            for less in sorted({0, 1, 2, 3, 9, 17, 100, most // 2, most - 1, most}):
+                for shorter, window in ((length, 0), (length // 3, 0), (100, 0), (length, 50), (length, 1000)):
+                    if not (0 < fewer <= entries and 0 <= less <= most):
+                        continue
+                    b = batch(qi, entries=fewer, tokens=fewer * less, most=less)
+                    assert library.qi_kv_attention_workspace(ctypes.byref(c), ctypes.byref(b), heads, shorter, ctypes.byref(size)) == 0 and size.value <= bound
+                    call = qi.qi_kv_attention(layer=1, heads=heads, q=256, ld_q=width, y=512, ld_y=width, lse=0, scale=0.1, causal=1, window=window, max_length=shorter)
+                    status = library.qi_kv_attention_ex(ctypes.byref(c), ctypes.byref(p), ctypes.byref(b), ctypes.byref(call), 256, bound, None)
+                    assert status != INVALID, (fewer, less, shorter, window)
+
+
 def test_unfit_page_lists(qi):
     library, c, p = qi.lib(), ctypes.byref(cache(qi)), ctypes.byref(pages(qi))
     size = ctypes.c_size_t(0)

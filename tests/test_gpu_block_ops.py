@@ -211,6 +211,34 @@ def test_calls_of_different_shapes_share_a_workspace(qi):
             assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm(), (counts, heads)
 
 
+def test_a_workspace_for_the_largest_batch_serves_the_smaller_ones(qi):
+    lengths, dim, heads = [5000, 900, 400, 70] * 10, 128, 8
+    store = Store(qi, 39, lengths)
+    largest = store.batch(list(range(40)), [900] * 40)
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, largest, heads, 5000), dtype=torch.uint8, device="cuda")
+    for slots, counts in ((list(range(40)), [40] * 40), ([0], [900]), ([0, 2], [300, 300]), ([4], [5]), (list(range(40)), [1] * 40), ([8], [1]), ([0, 4, 8], [4, 2, 3])):
+        q = (torch.randn(sum(counts), heads, dim, device="cuda") * 1.5).half()
+        y, batch = torch.full_like(q, float("nan")), store.batch(slots, counts)
+        for window in (0, 600):
+            assert qi.kv_attention_ex(store.cache, store.pages, batch, 1, q, heads * dim, y, heads * dim, heads, dim ** -0.5, 5000, window=window, workspace=workspace) == 0
+            settled(qi)
+            exact, _ = attend_exact(store, q, slots, counts, heads, dim ** -0.5, True, window)
+            assert (y.double() - exact).norm() <= 2.0 ** -11 * exact.norm(), (counts, window)
+
+
+def test_the_example_serves_two_prompts_at_once(qi):
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("cached_block_two", os.path.join(entry.ROOT, "examples", "cached_block.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    server = example.Server(qi, example.Model(qi))
+    server.reserve([0, 1], [250, 262])
+    assert torch.isfinite(server.forward([0, 1], [250, 262], torch.randn(512, example.WIDTH, device="cuda"))).all()
+    assert all(word.item() == 0 for word in server.words)
+    settled(qi)
+
+
 def test_long_cache_is_split(qi):
     store = Store(qi, 3, [20011, 1, 9000], page=64)
     attend(qi, store, [0, 1, 2], [1, 1, 1], 8)
