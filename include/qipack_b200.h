@@ -485,7 +485,7 @@ int qi_kv_read_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_k
  *   y[r, h] = sum_j softmax_j(scale * q[r, h] . k[j, h / (heads / kv_heads)]) v[j, h / (heads / kv_heads)]
  * q and y [tokens, heads, head_dim] float16, ld_q and ld_y elements between rows (multiples of 8). Row i of an entry with
  * c tokens of a sequence of n stands at position p = n - c + i. `causal`: it sees tokens j <= p; `window` > 0: it sees
- * tokens j > p - window only. A row that sees nothing (no token, or p < 0) gives zeros. lse [tokens, heads] float32 or NULL
+ * tokens j > p - window only. A row that sees nothing (there is no token, or `causal` and p < 0) gives zeros. lse [tokens, heads] float32 or NULL
  * receives log sum_j exp(scale * q . k), -infinity for such a row, with which results over several caches can be
  * joined. Queries and weights enter the products as float16, codes exactly; all sums are float32. Tokens whose
  * page the table does not name soundly are hidden from all rows, an entry that is unsound leaves its rows of y and lse as they are, and the status word says so. max_length bounds the

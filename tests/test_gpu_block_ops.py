@@ -187,6 +187,15 @@ def test_rows_that_see_nothing(qi, heads):
     attend(qi, store, [0, 4], [1, 3], heads, causal=False)
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("counts", [[4, 5, 2], [40, 300, 30]])
+@pytest.mark.parametrize("window", [0, 2, 35])
+def test_more_queries_than_tokens_without_a_causal_mask(qi, counts, window, head_dim):
+    # rows before the first token see all of them, or with a window those that it reaches: zeros only where there are no tokens
+    y = attend(qi, Store(qi, 49, [2, 34, 0], head_dim=head_dim), [0, 1, 2], counts, 4, causal=False, window=window)
+    assert (y[: counts[0] + counts[1]] != 0).any(1).all() and (y[counts[0] + counts[1]:] == 0).all()
+
+
 @pytest.mark.parametrize("window", [0x7fffffff, 0x7fffffff - 4, 1 << 30])
 @pytest.mark.parametrize("counts", [[5, 6], [30, 290]])
 @pytest.mark.parametrize("causal", [False, True])
