@@ -282,6 +282,42 @@ def test_many_queries(qi):
     attend(qi, store, [1], [999], 14, window=300)
 
 
+@pytest.mark.parametrize("kv_heads,heads", [(1, 7), (2, 2), (4, 12)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 129), (False, 300), (True, 1)])
+def test_many_queries_of_64_channels(qi, kv_heads, heads, causal, window):
+    # several tiles of rows, which end within a tile of tokens, within a page and within a group of heads
+    store = Store(qi, 51, [1100, 900, 257, 40], kv_heads=kv_heads, head_dim=64, page=32)
+    attend(qi, store, [0, 1, 2, 3], [1100, 333, 257, 40], heads, causal=causal, window=window)
+    attend(qi, store, [2, 1], [129, 513], heads, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_many_queries_over_a_long_cache_in_pieces(qi, head_dim, page):
+    store = Store(qi, 53, [20011, 9000, 130], page=page, head_dim=head_dim, kv_heads=1)
+    for causal, window in ((True, 0), (False, 0), (True, 5000), (False, 700)):
+        attend(qi, store, [0, 1, 2], [150, 33, 130], 2, causal=causal, window=window)
+        attend(qi, store, [1], [20], 1, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("counts", [[1, 1], [3, 8], [90, 200]])
+def test_queries_that_are_not_finite_spoil_their_own_rows_only(qi, counts, head_dim):
+    store, heads, tokens = Store(qi, 55, [700, 260], head_dim=head_dim), 4, sum(counts)
+    q = (torch.randn(tokens, heads, head_dim, device="cuda") * 1.5).half()
+    exact, exact_lse = attend_exact(store, q, [0, 1], counts, heads, head_dim ** -0.5, True, 0)
+    spoilt = torch.zeros(tokens, heads, dtype=torch.bool, device="cuda")
+    for i, (token, head) in enumerate([(0, 1), (tokens - 1, 0), (tokens - 1, 3), (tokens // 2, 2)]):
+        q[token, head, 5 * i] = (float("nan"), float("inf"), float("-inf"), float("nan"))[i]
+        spoilt[token, head] = True
+    y, lse, batch = torch.zeros_like(q), torch.zeros(tokens, heads, device="cuda"), store.batch([0, 1], counts)
+    workspace = torch.zeros(qi.kv_attention_workspace(store.cache, batch, heads, 700), dtype=torch.uint8, device="cuda")
+    assert qi.kv_attention_ex(store.cache, store.pages, batch, 1, q, heads * head_dim, y, heads * head_dim, heads, head_dim ** -0.5, 700, lse=lse, workspace=workspace) == 0
+    settled(qi)
+    assert y[spoilt].isnan().all()
+    assert (y[~spoilt].double() - exact[~spoilt]).norm() <= 2.0 ** -11 * exact[~spoilt].norm() and (lse.double() - exact_lse)[~spoilt].abs().max() <= 1e-5
+
+
 def test_strides_streams_and_loose_bounds(qi):
     store = Store(qi, 5, [500, 300])
     stream = torch.cuda.Stream()
@@ -519,6 +555,31 @@ def test_append_of_zeros_and_of_extremes(qi):
     assert qi.kv_attention_ex(store.cache, store.pages, store.batch([0], [1]), 1, torch.ones_like(y), 256, y, 256, 2, 1.0, 16) == 0
     settled(qi)
     assert (y == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_append_of_blocks_of_every_magnitude(qi, dtype):
+    # a block each from the largest numbers down to those whose scale is no normal float32, or rounds to zero; then eight more tokens for each,
+    # of which every other block's are larger, so that the earlier ones are rounded again by what may be a quotient of such scales
+    sizes = [3e37, 1e30, 1.0, 2e-34, 1.2e-34, 1e-35, 1e-36, 1e-38, 1e-40, 1e-42, 2e-44, 0.0] if dtype == torch.float32 else [1e4, 1.0, 1e-3, 1e-4, 6e-6, 6e-8, 0.0]
+    count = len(sizes)
+    a, b = (Store(qi, 57, [8] * count, page=16, fill=False) for _ in range(2))
+    width, code = a.kv_heads * a.head_dim, qi.DTYPE_F16 if dtype == torch.float16 else qi.DTYPE_F32
+    g = torch.Generator(device="cuda").manual_seed(58)
+    for step in range(2):
+        rows = torch.randn(8 * count, 2 * width, device="cuda", generator=g).double().clamp(-4, 4)
+        for i, size in enumerate(sizes):
+            rows[8 * i:8 * i + 8] *= size * (2.5 if step and i % 2 else 1.0)
+        rows = rows.to(dtype)
+        for store in (a, b):
+            store.lengths_list = [8 * (step + 1)] * count
+            store.lengths.fill_(8 * (step + 1))
+        append_plain(b, {"k": rows[:, :width].reshape(-1, a.kv_heads, a.head_dim), "v": rows[:, width:].reshape(-1, a.kv_heads, a.head_dim)}, list(range(count)), [8] * count)
+        assert qi.kv_append_ex(a.cache, a.pages, a.batch(list(range(count)), [8] * count), 1, rows, rows[:, width:], code, 2 * width, 2 * width) == 0
+        settled(qi)
+        assert same_bytes(a, b), step
+    if dtype == torch.float32:  # the blocks reach what is no normal number; float16 ones do not (2^-24 / 127)
+        assert min(float(a.scales["k"][1, a.table[i, 0]].max()) for i, size in enumerate(sizes) if size) < 2.0 ** -126
 
 
 @pytest.mark.parametrize("kv_heads", [1, 4, 9])
@@ -902,6 +963,27 @@ def test_norm_of_rows_without_spread(qi):
     assert (y[:2] == 0).all()
     exact = norm_exact(x[2:].double(), qi.NORM_LAYER, 1e-6, qi)
     assert (y[2:].double() - exact).abs().max() <= 2.0 ** -10  # a mean of 1e4 in 32 bits is known to 2^-11 of a deviation
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,width", [(700, 512), (900, 4096), (5, 16384)])
+def test_rows_that_are_not_finite_spoil_themselves_only(qi, kind, rows, width):
+    kind = qi.NORM_LAYER if kind == "layer" else qi.NORM_RMS
+    x, branch, weight = torch.randn(rows, width, device="cuda"), torch.randn(rows, width, device="cuda").half(), torch.randn(width, device="cuda")
+
+    def call():
+        y, out = torch.empty(rows, width, device="cuda"), torch.empty(rows, width, device="cuda")
+        assert qi.gated_norm_ex(qi.GatedNorm(rows, width, kind=kind, residual=x, branch=branch, branch_dtype=qi.DTYPE_F16, branch_norm=True, weight=weight, residual_out=out, y=y)) == 0
+        settled(qi)
+        return y, out
+
+    clean = call()
+    x[1, 7], branch[rows - 2, 100], x[rows // 2, width - 1] = float("nan"), float("inf"), float("-inf")
+    spoilt = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    spoilt[[1, rows - 2, rows // 2]] = True
+    for now, before in zip(call(), clean):
+        assert torch.equal(now[~spoilt], before[~spoilt])
+        assert now[spoilt].isfinite().all(1).logical_not().all()
 
 
 # ---- together ----------------------------------------------------------------------------------------------------------
