@@ -471,7 +471,8 @@ typedef struct {
  * lengths already count them, and no other sequence holds those pages. A block of 16 tokens and one head has
  *   scale = max |x| * (1 / 127) of its new tokens, or the scale of its earlier tokens if that is more,
  *   code  = rint(x / scale) + 128, earlier tokens again as rint((code - 128) * (old scale / scale)) + 128,
- * all in float32, ties to even. Writing the same tokens again changes nothing. An infinity or a NaN is held as 0, and the
+ * all in float32, ties to even. Writing the same tokens again changes nothing; writing others
+ * in their place rounds the block's earlier tokens again whenever its scale grows, by half a step of the new one at most, and a scale never falls while they are there. An infinity or a NaN is held as 0, and the
  * status word says so (0x0006C002). `most` may be any bound here: blocks of 16 that
  * `most` tokens, or the tokens of a row of the table if they are fewer, touch, times kv_heads, are at most 2^30 - 2. */
 int qi_kv_append_ex(const qi_kv_cache *cache, const qi_kv_pages *pages, const qi_kv_batch *batch, int layer, const void *k,

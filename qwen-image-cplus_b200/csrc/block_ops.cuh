@@ -53,7 +53,8 @@ kv::Cache layer_of(const qi_kv_cache *cache, int layer) {
 kv::Tables tables_of(const qi_kv_pages *pages) { return {pages->table, pages->lengths, pages->references, pages->sequences, pages->table_pages}; }
 kv::Batch batch_of(const qi_kv_batch *batch) { return {batch->slots, batch->offsets, batch->entries, batch->tokens, batch->most, batch->shortage}; }
 
-// A launch of any grid, overlapped with the kernel before it.
+// A launch of any grid. It may start while the kernel before it in the stream ends, if that one calls grid_release() (the packed linears do; the kernels of this
+// file do not, so behind one another they start when the one before has ended).
 template <typename... Parameters, typename... Arguments>
 int launch_grid(void (*kernel)(Parameters...), dim3 grid, int threads, int smem_bytes, void *stream, const Arguments &...arguments) {
     cudaLaunchConfig_t config = {};

@@ -105,7 +105,7 @@ template <int DIM, int TILES>
 struct Decode {
     // CTAs to an SM, rounds of a ring, and rounds that are worth a CTA of their own (joining a piece costs as much). 64 sequences of 2048 to
     // 8192 tokens, 8 heads: 128 channels, three CTAs with rings of two 124 us, two with three the same, but 131071 tokens of one 70 and 62;
-    // 64 channels 78 with three, 89 with two. With 16 rows two rounds, so that two CTAs fit: 163 us, 234 with one.
+    // 64 channels 78 with three, 89 with two. With 16 rows two rounds, so that two CTAs fit: 152 us, 234 with one.
     static constexpr int CTAS = DIM == 64 ? 3 : 2, LEAST_ROUNDS = TILES == 1 ? 2 : 4;
     static constexpr int STAGES = (DIM == 64 ? 4 : 3) - (TILES == 1 ? 0 : 1), STAGE_BYTES = 2 * STEP * DIM + 32;  // codes of keys, of values, scales
     struct Join {
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, Decode<DIM, TILES>::CTAS) deco
     int head = static_cast<int>(divide(first_round - unit_round, span.rounds)), r = static_cast<int>(first_round - unit_round - static_cast<long long>(head) * span.rounds);
     unit_round += static_cast<long long>(head) * span.rounds;
 
-    // Each warp has a ring of STAGES steps of its own in shared memory, filled by 16-byte asynchronous copies, 16 KB of them under way at
-    // any time. Pieces of a row are stored where eight lanes that read together meet no bank twice (DIM 64, values: two of them do).
+    // Each warp has a ring of STAGES steps of its own in shared memory, filled by 16-byte asynchronous copies, all rounds but one of
+    // them under way at any time: 16 KB with 128 channels, 12 with 64, 8 with 16 rows. Pieces of a row are stored where eight lanes that read together meet no bank twice (DIM 64, values: two of them do).
     uint8_t *ring = smem + warp * (STAGES * STAGE_BYTES);
     // what is fetched next: it runs STAGES - 1 rounds ahead
     Span ahead = span;

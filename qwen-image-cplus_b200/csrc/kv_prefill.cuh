@@ -18,7 +18,8 @@
 // maximum taken, O rescaled (which waits for the product before) and the pass repeated. So no weight is more than 2^15 in float16, and
 // all its digits are kept down to 2^-21 of the largest; sums are float32. Only the first tile pays for a pass over its maximum.
 //
-// Two guided sequences of 4096 and about 1600 queries over 4173 tokens, 32 heads: 463 us, 890 TFLOP/s; one round of CTAs over 65536 tokens 1030. A
+// Two guided sequences, 4096 queries over 4173 tokens and 2691 over 2999, 32 heads: 505 us, 816 TFLOP/s, call after call (463 us and 890 in the first
+// hundred calls, before the power limit); one round of CTAs over 65536 tokens 1030. A
 // tile takes a CTA 2.3 us, of which the products alone would be 1.6 (two thirds of the tensor cores' rate: Q and K from shared memory are
 // 128 bytes a clock, and the widened codes are written beside them); the rest is the chain scores - weights - product - next scores,
 // which two halves of rows overlap and do not fill (issue slots 38 %, special functions 40 %, tensor cores 42 % busy). A CTA starts for 5 us

@@ -557,6 +557,40 @@ def test_append_of_zeros_and_of_extremes(qi):
     assert (y == 0).all()
 
 
+def test_what_rewriting_costs_a_prefix_in_the_same_block(qi):
+    # Ten steps write other tokens behind 5 earlier ones of their block. Each growth of a scale rounds those once more, by half a step of the new scale;
+    # a whole block ahead of them stays bit for bit; and what is written last is as near as a single rounding makes it.
+    prefix, image, steps = 21, 30, 10
+    store = Store(qi, 59, [prefix], page=16, spare=8, table_extra=2, fill=False)
+    width = store.kv_heads * store.head_dim
+    rows, kv = make_kv(store, prefix, torch.float32, 60, spread=0.0)
+    assert qi.kv_append_ex(store.cache, store.pages, store.batch([0], [prefix]), 1, rows, rows[:, width:], qi.DTYPE_F32, 2 * width, 2 * width) == 0
+    told, workspace = ints([9]), torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda")
+    assert qi.kv_pages_reserve_ex(store.cache, store.pages, ints([0]), ints([image]), 1, told, workspace) == 0
+    settled(qi)
+    assert told.item() == 0
+    first, growths, scale = store.values("k", 0)[:16].clone(), torch.ones(store.kv_heads, device="cuda"), None
+    for step in range(steps):
+        new, new_kv = make_kv(store, image, torch.float32, 61 + step, spread=0.5)
+        assert qi.kv_append_ex(store.cache, store.pages, store.batch([0], [image]), 1, new, new[:, width:], qi.DTYPE_F32, 2 * width, 2 * width) == 0
+        settled(qi)
+        store.lengths_list = [prefix + image]
+        now = store.scales["k"][1, int(store.table[0, 1]), :, 0].clone()
+        growths += 1 if scale is None else (now > scale)  # the first step's counts, whether it grew or not
+        assert scale is None or (now >= scale).all()
+        scale = now
+        held, bound = store.values("k", 0), (0.5 + 1e-4) * scale.double()
+        assert torch.equal(held[:16], first)
+        assert ((held[16:prefix] - kv["k"][16:].double()).abs() <= (growths * bound)[:, None]).all()
+        assert ((held[prefix:32] - new_kv["k"][:32 - prefix].double()).abs() <= bound[:, None]).all()
+    # appended again from the block's start, the prefix has its digits back
+    both = torch.cat([rows[16:], new])
+    assert qi.kv_append_ex(store.cache, store.pages, store.batch([0], [prefix - 16 + image]), 1, both, both[:, width:], qi.DTYPE_F32, 2 * width, 2 * width) == 0
+    settled(qi)
+    scale = store.scales["k"][1, int(store.table[0, 1]), :, 0].double()
+    assert ((store.values("k", 0)[16:prefix] - kv["k"][16:].double()).abs() <= ((0.5 + 1e-4) * scale)[:, None]).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_append_of_blocks_of_every_magnitude(qi, dtype):
     # a block each from the largest numbers down to those whose scale is no normal float32, or rounds to zero; then eight more tokens for each,
