@@ -184,21 +184,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_kernel(PageTables t, const 
         int *row = t.table + static_cast<long long>(child) * t.table_pages;
         const int have = pages_of(work.held[i], t.page_shift), whole = work.held[i] >> t.page_shift;
         const int before = min(pages_of(max(t.lengths[child], 0), t.page_shift), t.table_pages);
+        // of the last page, which is copied; a parent that has none there leaves its child none either, and not what a free page happens to hold
+        const int from = have > whole ? work.rows[static_cast<long long>(i) * t.table_pages + whole] : -1;
+        const bool there = from >= 0 && from < t.pages;
         for (int j = lane; j < max(have, before); j += 32) {
             const int gone = j < before ? row[j] : -1;
             if (gone >= 0 && gone < t.pages) atomicSub(t.references + gone, 1);
             int page = -1;
             if (j < whole) page = work.rows[static_cast<long long>(i) * t.table_pages + j];
-            else if (j < have) page = work.moved[work.targets[i]];
+            else if (j < have && there) page = work.moved[work.targets[i]];
             row[j] = page;
         }
         __syncwarp();
         if (lane == 0) {
             t.lengths[child] = work.held[i];
             if (have > whole) {
-                const int rank = work.targets[i], from = work.rows[static_cast<long long>(i) * t.table_pages + whole];
-                t.references[work.moved[rank]] = 1;
-                work.sources[rank] = from >= 0 && from < t.pages ? from : work.moved[rank];
+                const int rank = work.targets[i];
+                if (there) t.references[work.moved[rank]] = 1;
+                work.sources[rank] = there ? from : work.moved[rank];
             }
         }
     }

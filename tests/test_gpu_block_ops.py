@@ -856,6 +856,33 @@ def test_pages_that_do_not_suffice_change_nothing(qi):
     ledger.check(start)
 
 
+@pytest.mark.parametrize("fault", [-1, 0x7fffffff])
+def test_a_fork_of_a_sequence_whose_last_page_is_missing(qi, fault):
+    # the child has no page there either, not a free one with what it last held; the other children of the call are as always
+    store = Store(qi, 63, [75, 40, 10, 5], page=32, spare=6, table_extra=2)
+    store.table[0, 2] = fault
+    rows, references, start = store.table.tolist(), store.references.tolist(), pool_copy(store)
+    told, workspace = ints([9]), torch.empty(qi.kv_pages_workspace(store.cache, store.pages), dtype=torch.uint8, device="cuda").fill_(0xA5)
+    assert qi.kv_pages_fork_ex(store.cache, store.pages, ints([0, 1]), ints([2, 3]), 2, told, workspace) == 0
+    assert qi.kernel_status() >> 12 == 0x6C
+    assert told.item() == 0 and store.lengths.tolist() == [75, 40, 75, 40]
+    table, now = store.table.tolist(), store.references.tolist()
+    free = [p for p, n in enumerate(references) if n == 0]
+    assert table[:2] == rows[:2]
+    assert table[2] == rows[0][:2] + [-1] * (len(rows[0]) - 2)
+    assert table[3][0] == rows[1][0] and table[3][1] in free[:2] and table[3][2:] == [-1] * (len(rows[0]) - 2)
+    for p in rows[0][:2] + [rows[1][0]]:
+        references[p] += 1
+    for p in (rows[2][0], rows[3][0]):
+        references[p] -= 1
+    references[table[3][1]] = 1
+    assert now == references
+    for which in "kv":
+        expected = start[which + "c"].clone()
+        expected[:, table[3][1]] = expected[:, rows[1][1]]
+        assert torch.equal(store.codes[which], expected)
+
+
 def test_reserving_for_a_sequence_twice_stays_within_its_row(qi):
     # against the rules, and what it gives is not defined, but other rows, what lies behind the table and other pages are left alone
     page, sequences, width = 16, 40, 3
